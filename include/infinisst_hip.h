@@ -287,6 +287,50 @@ int isst_op_attn_combine(const float* partial, uint16_t* out, int heads, int row
 int isst_op_gemm_attn_merge(const float* partial, int n_splits, const uint16_t* packed, const uint16_t* res, int64_t ldres, uint16_t* out,
                             int64_t ldo, int M, int N, int K, void* hip_stream);
 
+/* ---- a decode step of many streams over one prompt: shared-prefix attention, an adapter per row, drafted tokens.  All pointers are DEVICE pointers of the
+ * CURRENT device, work is enqueued on `hip_stream` and nothing waits for it (graph capture is fine); workspaces belong to one call until its work is done. ---- */
+/* Attention of `rows` query rows of `seqs` sequences that share a prefix of prefix_len keys in front of keys of their own (the batched form of patch_llm.py:320-329's
+ * softmax(q k^T) v, keys already rotated).  Sequence b owns rows row_starts[b] .. row_starts[b + 1] - 1 (NULL: rows / seqs each) = its newest positions: row t of n
+ * sees every prefix key and the own keys 0 .. tail_lens[b] - n + t.  A row that sees no key gives zeros; rows outside every sequence are left as they were.
+ * Strides in elements, every row of head_dim elements contiguous and 16-byte aligned.  tail_lens is read as clamped to 0 .. tail_cap, row_starts (non-decreasing)
+ * to 0 .. rows: nothing outside the arrays is touched whatever they hold. */
+typedef struct isst_prefix_attn {
+    const uint16_t* q;              /* [rows][heads][head_dim] */
+    const uint16_t *k_prefix, *v_prefix; /* [kv_heads][prefix_len][head_dim] */
+    const uint16_t *k_tail, *v_tail;     /* [seqs][kv_heads][tail_cap][head_dim] */
+    const int* tail_lens;           /* [seqs] */
+    const int* row_starts;          /* [seqs + 1] or NULL */
+    uint16_t* out;                  /* [rows][heads][head_dim] */
+    int64_t q_row, q_head, out_row, out_head;
+    int64_t kp_head, kp_key, vp_head, vp_key;
+    int64_t kt_seq, kt_head, kt_key, vt_seq, vt_head, vt_key;
+    int rows, seqs, max_rows;       /* max_rows: most rows of one sequence (sizes the launch; 0 = unknown, more than that is still computed) */
+    int heads, kv_heads, head_dim;  /* heads % kv_heads == 0; head_dim 64 or 128 */
+    int prefix_len, tail_cap;
+    float scale;                    /* > 0 */
+} isst_prefix_attn;
+int64_t isst_op_prefix_attention_workspace(const isst_prefix_attn* a); /* bytes (16-byte aligned memory), < 0: bad arguments */
+int isst_op_prefix_attention(const isst_prefix_attn* a, void* workspace, int64_t workspace_bytes, void* hip_stream);
+/* out[m] = bf16(A[m] W^T + scales[a] * (A[m] down[a]^T) up[a]^T), a = row_adapter[m]; a row whose a is outside 0 .. n_adapters - 1 has no adapter.  packed:
+ * isst_op_pack_weight of W [N][K]; down [n_adapters][rank][K], up [n_adapters][N][rank] bf16 contiguous; rank a multiple of 8 up to 128; K % 32 == 0.
+ * Sums stay in fp32, one rounding at the end.  F.linear next to per-request adapters; the reference has one set of weights per language pair instead. */
+int64_t isst_op_gemm_lora_workspace(int M, int N, int K, int rank, int n_adapters);
+int isst_op_gemm_lora(const uint16_t* A, int64_t lda, const uint16_t* packed, const uint16_t* down, const uint16_t* up, const float* scales,
+                      const int* row_adapter, int n_adapters, int rank, uint16_t* out, int64_t ldo, int M, int N, int K, void* workspace,
+                      int64_t workspace_bytes, void* hip_stream);
+/* Speculative verification.  Per stream b: drafted tokens drafts[b][0 .. n - 1], n = n_drafts[b] (NULL: max_drafts), the model's processed scores target
+ * [streams][max_drafts + 1][vocab] (row i: the scores after i accepted drafts), the draft's scores draft_scores [streams][max_drafts][vocab] (NULL: a draft without a
+ * distribution, i.e. probability one).  With p, q = softmax of the rows in 64 bits: draft i is accepted while uniforms[b][i] * q_i(x_i) < p_i(x_i); after the first refusal the
+ * next token is drawn from max(p_i - q_i, 0) (from p_i where nothing is left), after n acceptances from p_n, by inverse CDF in vocabulary order at
+ * uniforms[b][max_drafts] (isst_op_warp_sample's rule: first entry whose running sum exceeds u * total).  uniforms NULL: greedy -- a draft is accepted while it is its row's
+ * argmax (lowest index on ties), then that argmax follows.  tokens[b][0 .. counts[b] - 1] = the accepted drafts and the drawn token, -1 behind them.  counts[b] = -1 (all
+ * tokens -1): n_drafts[b], a drafted token or a uniform that decides is out of range, or a row that decides holds NaN, +inf or no finite score.  Rows behind the first refusal do not
+ * matter.  target_stream / target_row / draft_stream / draft_row: strides in elements (a row is contiguous). */
+int64_t isst_op_verify_drafts_workspace(int streams, int max_drafts, int vocab);
+int isst_op_verify_drafts(const float* target, int64_t target_stream, int64_t target_row, const float* draft_scores, int64_t draft_stream, int64_t draft_row,
+                          const int* drafts, const int* n_drafts, const double* uniforms, int streams, int max_drafts, int vocab, int* tokens, int* counts,
+                          void* workspace, int64_t workspace_bytes, void* hip_stream);
+
 #ifdef __cplusplus
 }
 #endif

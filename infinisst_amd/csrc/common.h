@@ -113,6 +113,7 @@ enum GemmEpi {
     EPI_F32 = 6,        // out(fp32) = bf16-rounded acc
     EPI_PARTIAL = 7,    // split-K slab: out(fp32)[slice][M][N] = raw partial sum (gemm_mid.hip; reduced by rmsnorm_reduce)
     EPI_SWIGLU8 = 8,    // SwiGLU on SELF-PAIRED tiles (gemm.hip, one-row passes): tile t = gate rows 8t..8t+7 | up rows 8t..8t+7 (launch_pack_weight_half): out[8t + c] as EPI_SWIGLU
+    EPI_RAW = 9,        // out(fp32) = acc, unrounded (gemm.hip only; a consumer adds to it: lora.hip)
 };
 
 // launchers (defined in the kernel .hip files; all asynchronous on `stream`)

@@ -253,3 +253,103 @@ extern "C" int isst_op_gemm_attn_merge(const float* partial, int n_splits, const
     return launch_gemm(g, reinterpret_cast<hipStream_t>(hip_stream));
 }
 
+// ---- a decode step of many streams over one prompt (prefix_attn.hip, lora.hip, verify.hip) ----
+static inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+static bool prefix_attention_ok(const isst_prefix_attn* a) {
+    if (!a || a->rows < 0 || a->seqs < 0 || a->max_rows < 0 || a->heads < 1 || a->kv_heads < 1 || a->heads % a->kv_heads || (a->head_dim != 64 && a->head_dim != 128) ||
+        a->prefix_len < 0 || a->tail_cap < 0 || !(a->scale > 0.f) || !(a->scale < INFINITY))
+        return false;
+    if ((int64_t)a->rows * a->heads > (1 << 30) || (a->rows > 0 && a->seqs < 1)) return false;
+    if (!a->row_starts && a->seqs > 0 && a->rows % a->seqs) return false;
+    if (a->rows == 0) return true;
+    if (!a->q || !a->out || !a->tail_lens || !aligned16(a->q) || !aligned16(a->out)) return false;
+    int64_t strides = a->q_row | a->q_head | a->out_row | a->out_head;
+    if (a->prefix_len > 0) {
+        if (!a->k_prefix || !a->v_prefix || !aligned16(a->k_prefix) || !aligned16(a->v_prefix)) return false;
+        strides |= a->kp_head | a->kp_key | a->vp_head | a->vp_key;
+    }
+    if (a->tail_cap > 0) {
+        if (!a->k_tail || !a->v_tail || !aligned16(a->k_tail) || !aligned16(a->v_tail)) return false;
+        strides |= a->kt_seq | a->kt_head | a->kt_key | a->vt_seq | a->vt_head | a->vt_key;
+    }
+    if (strides & 7) return false;
+    // two outputs never share memory
+    return (a->heads == 1 || a->out_head >= a->head_dim) && (a->rows == 1 || a->out_row >= (a->heads - 1) * a->out_head + a->head_dim);
+}
+extern "C" int64_t isst_op_prefix_attention_workspace(const isst_prefix_attn* a) { return prefix_attention_ok(a) ? (a->rows ? prefix_attention_workspace(*a) : 0) : ISST_ERR_ARG; }
+extern "C" int isst_op_prefix_attention(const isst_prefix_attn* a, void* workspace, int64_t workspace_bytes, void* hip_stream) {
+    if (!prefix_attention_ok(a)) return ISST_ERR_ARG;
+    if (a->rows == 0) return ISST_OK;
+    const int64_t need = prefix_attention_workspace(*a);
+    if (need > 0 && (!workspace || !aligned16(workspace))) return ISST_ERR_ARG;
+    if (workspace_bytes < need) return ISST_ERR_NOMEM;
+    return launch_prefix_attention(*a, workspace, reinterpret_cast<hipStream_t>(hip_stream));
+}
+
+// K slices of the base product: fp32 slabs through the many-row kernels, the raw accumulator through the register-A one where they do not run
+static GemmArgs lora_base_args(const uint16_t* A, int64_t lda, const uint16_t* packed, float* base, int M, int N, int K) {
+    GemmArgs g{};
+    g.A = A; g.lda = lda; g.Wp = packed; g.out = base; g.N = round_up(N, 16); g.ldo = g.N; g.out_batch = (long)M * g.N;
+    g.M = M; g.K = K; g.batch = 1; g.n_valid = N;
+    g.epi = EPI_PARTIAL;
+    g.ksplit = M > 12 ? pick_ksplit(K, g.N, M, 1L << 28) : 1;
+    if (gemm_mid_supported(g) || gemm_tiled_supported(g)) return g;
+    g.ksplit = 1;
+    if (gemm_mid_supported(g) || gemm_tiled_supported(g)) return g;
+    g.epi = EPI_RAW;
+    return g;
+}
+static bool lora_ok(int M, int N, int K, int rank, int n_adapters) {
+    return M >= 0 && N >= 1 && N <= (1 << 24) && K >= 32 && K % 32 == 0 && K <= (1 << 24) && rank >= 8 && rank <= 128 && rank % 8 == 0 && n_adapters >= 1 &&
+           (int64_t)M * N < (1L << 30) && (int64_t)M * K < (1L << 29);
+}
+extern "C" int64_t isst_op_gemm_lora_workspace(int M, int N, int K, int rank, int n_adapters) {
+    if (!lora_ok(M, N, K, rank, n_adapters)) return ISST_ERR_ARG;
+    const GemmArgs g = lora_base_args(nullptr, K, nullptr, nullptr, M, N, K);
+    return ((int64_t)g.ksplit * M * g.N + lora_t_floats(M, N, K, rank, n_adapters)) * (int64_t)sizeof(float);
+}
+extern "C" int isst_op_gemm_lora(const uint16_t* A, int64_t lda, const uint16_t* packed, const uint16_t* down, const uint16_t* up, const float* scales,
+                                 const int* row_adapter, int n_adapters, int rank, uint16_t* out, int64_t ldo, int M, int N, int K, void* workspace,
+                                 int64_t workspace_bytes, void* hip_stream) {
+    if (!lora_ok(M, N, K, rank, n_adapters)) return ISST_ERR_ARG;
+    if (M == 0) return ISST_OK;
+    if (!A || !packed || !down || !up || !scales || !row_adapter || !out || !workspace || lda < K || lda % 8 || (int64_t)M * lda >= (1L << 29) || ldo < N || !aligned16(A) ||
+        !aligned16(packed) || !aligned16(down) || !aligned16(up) || !aligned16(workspace))
+        return ISST_ERR_ARG;
+    if (workspace_bytes < isst_op_gemm_lora_workspace(M, N, K, rank, n_adapters)) return ISST_ERR_NOMEM;
+    hipStream_t st = reinterpret_cast<hipStream_t>(hip_stream);
+    const GemmArgs g = lora_base_args(A, lda, packed, static_cast<float*>(workspace), M, N, K);
+    LoraArgs l{};
+    l.A = A; l.lda = lda; l.down = down; l.up = up; l.scales = scales; l.row_adapter = row_adapter;
+    l.base = static_cast<const float*>(workspace); l.ld_base = g.N; l.slabs = g.ksplit;
+    l.t = static_cast<float*>(workspace) + (int64_t)g.ksplit * M * g.N;
+    l.out = out; l.ldo = ldo; l.M = M; l.N = N; l.K = K; l.rank = rank; l.n_adapters = n_adapters;
+    int rc = launch_lora_down(l, st);
+    if (rc == ISST_OK) rc = launch_gemm(g, st);
+    if (rc == ISST_OK) rc = launch_lora_up(l, st);
+    return rc;
+}
+
+static bool verify_ok(int streams, int max_drafts, int vocab) {
+    return streams >= 0 && max_drafts >= 0 && vocab >= 1 && (int64_t)streams * (2 * (int64_t)max_drafts + 1) < (1 << 24);
+}
+extern "C" int64_t isst_op_verify_drafts_workspace(int streams, int max_drafts, int vocab) {
+    return verify_ok(streams, max_drafts, vocab) ? verify_workspace(streams, max_drafts, vocab) : ISST_ERR_ARG;
+}
+extern "C" int isst_op_verify_drafts(const float* target, int64_t target_stream, int64_t target_row, const float* draft_scores, int64_t draft_stream, int64_t draft_row,
+                                     const int* drafts, const int* n_drafts, const double* uniforms, int streams, int max_drafts, int vocab, int* tokens, int* counts,
+                                     void* workspace, int64_t workspace_bytes, void* hip_stream) {
+    if (!verify_ok(streams, max_drafts, vocab)) return ISST_ERR_ARG;
+    if (streams == 0) return ISST_OK;
+    if (!target || (max_drafts > 0 && !drafts) || !tokens || !counts || !workspace || !aligned16(workspace) || target_stream < 0 || target_row < 0 || draft_stream < 0 || draft_row < 0 ||
+        ((reinterpret_cast<uintptr_t>(target) | reinterpret_cast<uintptr_t>(draft_scores) | reinterpret_cast<uintptr_t>(drafts) | reinterpret_cast<uintptr_t>(n_drafts) |
+          reinterpret_cast<uintptr_t>(tokens) | reinterpret_cast<uintptr_t>(counts)) & 3) || (reinterpret_cast<uintptr_t>(uniforms) & 7))
+        return ISST_ERR_ARG;
+    if (workspace_bytes < verify_workspace(streams, max_drafts, vocab)) return ISST_ERR_NOMEM;
+    VerifyArgs v{};
+    v.target = target; v.target_stream = target_stream; v.target_row = target_row;
+    v.draft = max_drafts > 0 ? draft_scores : nullptr; v.draft_stream = draft_stream; v.draft_row = draft_row;
+    v.drafts = drafts; v.n_drafts = n_drafts; v.uniforms = uniforms; v.streams = streams; v.max_drafts = max_drafts; v.vocab = vocab;
+    v.tokens = tokens; v.counts = counts; v.workspace = workspace;
+    return launch_verify(v, reinterpret_cast<hipStream_t>(hip_stream));
+}

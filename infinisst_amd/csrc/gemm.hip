@@ -404,6 +404,8 @@ __global__ __launch_bounds__(AMODE == 3 ? 512 : 1024) void gemm_skinny_kernel(Ge
         if (row >= g.M || col >= g.n_valid) continue;
         if constexpr (EPI == EPI_F32) {
             reinterpret_cast<float*>(g.out)[b * g.out_batch + (long)row * g.ldo + col] = bfr(s);
+        } else if constexpr (EPI == EPI_RAW) {
+            reinterpret_cast<float*>(g.out)[b * g.out_batch + (long)row * g.ldo + col] = s;
         } else {
             float v;
             if constexpr (EPI == EPI_NONE) v = s;
@@ -505,7 +507,7 @@ int launch_gemm(const GemmArgs& g, hipStream_t stream) {
     }
     // 65..256 rows against a long weight stream (decode passes of many streams / streams x beams): weights read once, deep register rings
     if (!g_force_skinny && gemm_wide_supported(g) && gemm_wide_preferred(g)) return launch_gemm_wide(g, stream);
-    if (!g.attn_partial && gemm_tiled_supported(g) && !g_force_skinny) {
+    if (!g.attn_partial && g.epi != EPI_RAW && gemm_tiled_supported(g) && !g_force_skinny) {
         const bool ok = (g.epi != EPI_BIAS && g.epi != EPI_BIAS_GELU && g.epi != EPI_BIAS_RES) || g.bias;
         if (g.epi == EPI_PARTIAL ? g.ksplit < 1 : g.ksplit > 1) return ISST_ERR_ARG;
         if (!ok || ((g.epi == EPI_RES || g.epi == EPI_BIAS_RES) && !g.res) || (g.epi == EPI_SWIGLU && g.N % 32)) return ISST_ERR_ARG;
@@ -520,6 +522,7 @@ int launch_gemm(const GemmArgs& g, hipStream_t stream) {
         case EPI_BIAS_RES: return (g.res && g.bias) ? launch_epi<EPI_BIAS_RES>(g, stream) : ISST_ERR_ARG;
         case EPI_SWIGLU: return (g.N % 32 == 0) ? launch_epi<EPI_SWIGLU>(g, stream) : ISST_ERR_ARG;
         case EPI_F32: return launch_epi<EPI_F32>(g, stream);
+        case EPI_RAW: return launch_epi<EPI_RAW>(g, stream);
         case EPI_SWIGLU8: return (g.M <= 16 && g.batch == 1) ? launch_epi<EPI_SWIGLU8>(g, stream) : ISST_ERR_ARG;  // (the register-A GEMV only: the other kernels pair tiles)
     }
     return ISST_ERR_ARG;

@@ -262,3 +262,36 @@ int multinomial_without_replacement(const float* scores, long n, int k, const do
 double sample_uniform(uint64_t seed, int stream, int chunk, int step);
 int launch_sample_process(float* logits, long ld_logits, const SampleStream* ss, const int* ids_pool, const int* enc_pool, const int* suppress,
                           int n_suppress, float rep_penalty, int ngram, int enc_ngram, int n_rows, hipStream_t s);
+
+// ---- attention of a batch behind one shared prefix (prefix_attn.hip) ----
+struct isst_prefix_attn;  // include/infinisst_hip.h
+int64_t prefix_attention_workspace(const isst_prefix_attn& a);
+int launch_prefix_attention(const isst_prefix_attn& a, void* workspace, hipStream_t s);
+
+// ---- low-rank adapters per row beside a packed-weight GEMM (lora.hip) ----
+struct LoraArgs {
+    const bf16_t* A; long lda;           // [M][K]
+    const bf16_t *down, *up;             // [n_adapters][rank][K], [n_adapters][N][rank]
+    const float* scales;                 // [n_adapters]
+    const int* row_adapter;              // [M]
+    const float* base; long ld_base;     // [slabs][M][ld_base] fp32: K slices of A W^T
+    float* t;                            // lora_t_floats: down x per row, K slices of it
+    bf16_t* out; long ldo;
+    int M, N, K, rank, n_adapters, slabs;
+};
+int64_t lora_t_floats(int M, int N, int K, int rank, int n_adapters);
+int launch_lora_down(const LoraArgs& g, hipStream_t s);  // A, adapters -> t
+int launch_lora_up(const LoraArgs& g, hipStream_t s);    // base, t, adapters -> out
+
+// ---- verification of drafted tokens (verify.hip) ----
+struct VerifyArgs {
+    const float* target; long target_stream, target_row;
+    const float* draft; long draft_stream, draft_row;  // null: drafts without scores
+    const int *drafts, *n_drafts;                      // n_drafts null: max_drafts
+    const double* uniforms;                            // null: greedy
+    int streams, max_drafts, vocab;
+    int *tokens, *counts;
+    void* workspace;
+};
+int64_t verify_workspace(int streams, int max_drafts, int vocab);
+int launch_verify(const VerifyArgs& g, hipStream_t s);

@@ -64,6 +64,13 @@ class _StreamInfo(C.Structure):
                 ("enc_cache_len", C.c_int), ("chunks", C.c_int)]
 
 
+class _PrefixAttn(C.Structure):
+    _fields_ = ([(n, C.c_void_p) for n in ("q", "k_prefix", "v_prefix", "k_tail", "v_tail", "tail_lens", "row_starts", "out")]
+                + [(n, C.c_int64) for n in ("q_row", "q_head", "out_row", "out_head", "kp_head", "kp_key", "vp_head", "vp_key",
+                                            "kt_seq", "kt_head", "kt_key", "vt_seq", "vt_head", "vt_key")]
+                + [(n, C.c_int) for n in ("rows", "seqs", "max_rows", "heads", "kv_heads", "head_dim", "prefix_len", "tail_cap")] + [("scale", C.c_float)])
+
+
 # every symbol include/infinisst_hip.h declares
 EXPORTS = [
     "isst_create", "isst_destroy", "isst_last_error", "isst_load_weight", "isst_set_rope_tables", "isst_set_enc_position_table",
@@ -73,6 +80,7 @@ EXPORTS = [
     "isst_op_attn_combine", "isst_op_gemm_attn_merge", "isst_op_splice_map", "isst_op_embed_splice", "isst_op_enc_attention", "isst_op_llm_attention",
     "isst_generate", "isst_kv_evict", "isst_encode_speech", "isst_debug_tap", "isst_debug_read_kv", "isst_profile_begin", "isst_profile_begin_rows", "isst_profile_end", "isst_op_pack_weight", "isst_op_pack_gateup8",
     "isst_op_packed_elems", "isst_op_gemm", "isst_op_gemm_splitk_rmsnorm", "isst_op_gemm_splitk_fused", "isst_op_gemm_splitk_plain", "isst_op_gemm_norm_ssq", "isst_op_gemm_splitk_layernorm", "isst_op_set_gemm_tuning", "isst_op_set_attn_tuning", "isst_op_set_reduce_tuning", "isst_op_topk_rows", "isst_op_layernorm", "isst_op_rmsnorm", "isst_op_conv0", "isst_op_sample", "isst_op_warp", "isst_op_warp_sample", "isst_op_sample_uniform", "isst_op_multinomial_wor",
+    "isst_op_prefix_attention", "isst_op_prefix_attention_workspace", "isst_op_gemm_lora", "isst_op_gemm_lora_workspace", "isst_op_verify_drafts", "isst_op_verify_drafts_workspace",
 ]
 
 
@@ -148,6 +156,17 @@ def load_library(path: Optional[str] = None):
     lib.isst_op_sample_uniform.restype = C.c_double
     lib.isst_op_sample.argtypes = [C.c_void_p, C.c_int, C.c_void_p, C.c_int, C.c_void_p, C.c_int, C.c_void_p, C.c_int,
                                    C.c_float, C.c_int, C.c_int, C.c_void_p, C.c_void_p]
+    lib.isst_op_prefix_attention_workspace.argtypes = [C.POINTER(_PrefixAttn)]
+    lib.isst_op_prefix_attention_workspace.restype = C.c_int64
+    lib.isst_op_prefix_attention.argtypes = [C.POINTER(_PrefixAttn), C.c_void_p, C.c_int64, C.c_void_p]
+    lib.isst_op_gemm_lora_workspace.argtypes = [C.c_int] * 5
+    lib.isst_op_gemm_lora_workspace.restype = C.c_int64
+    lib.isst_op_gemm_lora.argtypes = [C.c_void_p, C.c_int64, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_int, C.c_int, C.c_void_p, C.c_int64,
+                                      C.c_int, C.c_int, C.c_int, C.c_void_p, C.c_int64, C.c_void_p]
+    lib.isst_op_verify_drafts_workspace.argtypes = [C.c_int] * 3
+    lib.isst_op_verify_drafts_workspace.restype = C.c_int64
+    lib.isst_op_verify_drafts.argtypes = [C.c_void_p, C.c_int64, C.c_int64, C.c_void_p, C.c_int64, C.c_int64, C.c_void_p, C.c_void_p, C.c_void_p, C.c_int, C.c_int,
+                                          C.c_int, C.c_void_p, C.c_void_p, C.c_void_p, C.c_int64, C.c_void_p]
     if path is None:
         _lib = lib
     return lib
@@ -715,3 +734,148 @@ def op_llm_attention(qkv: torch.Tensor, pos0: int, kpool: torch.Tensor, krpool: 
     if rc:
         raise IsstError(f"isst_op_llm_attention -> {rc}")
     return out
+
+
+# ---------------------------------------------------------------- a decode step of many streams over one prompt
+def _on_device(what: str, first: torch.Tensor, **tensors):
+    """Every given tensor lies on `first`'s GPU; returns that device (the ops below run there, on its current stream)."""
+    dev = first.device
+    if dev.type != "cuda":
+        raise IsstError(f"{what}: tensors must be on a GPU, got {dev}")
+    for name, t in tensors.items():
+        if t is not None and t.device != dev:
+            raise IsstError(f"{what}: {name} is on {t.device}, expected {dev}")
+    return dev
+
+
+def _expect(what: str, name: str, t: torch.Tensor, dtype: torch.dtype, shape=None, contiguous: bool = False):
+    if t.dtype != dtype or (shape is not None and tuple(t.shape) != tuple(shape)):
+        raise IsstError(f"{what}: {name} must be {dtype}{'' if shape is None else ' ' + str(tuple(shape))}, got {t.dtype} {tuple(t.shape)}")
+    if contiguous and not t.is_contiguous():
+        raise IsstError(f"{what}: {name} must be contiguous")
+
+
+def _row_strides(what: str, name: str, t: torch.Tensor) -> list:
+    """Strides of all dims but the last (0 where a dim has no second entry), for rows the kernels read 16 bytes at a time."""
+    if t.numel() == 0:
+        return [0] * (t.dim() - 1)
+    st = [s if n > 1 else 0 for s, n in zip(t.stride()[:-1], t.shape[:-1])]
+    if (t.stride(-1) != 1 and t.shape[-1] > 1) or t.data_ptr() % 16 or any(s % 8 for s in st):
+        raise IsstError(f"{what}: rows of {name} must be contiguous and 16-byte aligned (strides {t.stride()})")
+    return st
+
+
+def _launch(what: str, dev: torch.device, workspace_bytes: int, call):
+    """call(workspace pointer, bytes, stream) on `dev`'s current stream; the workspace is the caching allocator's, i.e. ordered by that stream."""
+    if workspace_bytes < 0:
+        raise IsstError(f"{what}: bad arguments ({workspace_bytes})")
+    if dev.index != torch.cuda.current_device():
+        with torch.cuda.device(dev):
+            return _launch(what, dev, workspace_bytes, call)
+    ws = torch.empty(workspace_bytes, dtype=torch.uint8, device=dev) if workspace_bytes else None
+    rc = call(None if ws is None else ws.data_ptr(), workspace_bytes, torch.cuda.current_stream().cuda_stream)
+    if rc:
+        raise IsstError(f"{what} -> {rc}")
+
+
+def op_prefix_attention(q: torch.Tensor, k_prefix: torch.Tensor, v_prefix: torch.Tensor, k_tail: torch.Tensor, v_tail: torch.Tensor, tail_lens: torch.Tensor,
+                        row_starts: Optional[torch.Tensor] = None, max_rows: int = 0, scale: Optional[float] = None, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Attention of sequences that share the keys k_prefix / v_prefix (kv_heads, P, D) in front of their own k_tail / v_tail (seqs, kv_heads, cap, D), of which
+    tail_lens (seqs, int32) are live.  q (rows, heads, D): sequence b's newest positions are rows row_starts[b] .. row_starts[b + 1] - 1 (int32, seqs + 1; None: as many
+    rows each); row t of n sees the prefix and the own keys 0 .. tail_lens[b] - n + t, a row without a key gives zeros, a row of no sequence is left as it was (in `out`;
+    undefined without).  max_rows: most rows of one sequence if the caller knows it (speed only).  bf16, D 64 or 128, keys already rotated; strided views are fine while
+    rows are 16-byte aligned.  scale: default D ** -0.5."""
+    what = "op_prefix_attention"
+    lib = load_library()
+    dev = _on_device(what, q, k_prefix=k_prefix, v_prefix=v_prefix, k_tail=k_tail, v_tail=v_tail, tail_lens=tail_lens, row_starts=row_starts, out=out)
+    if q.dim() != 3 or k_prefix.dim() != 3 or k_tail.dim() != 4:
+        raise IsstError(f"{what}: q (rows, heads, D), k_prefix (kv_heads, P, D), k_tail (seqs, kv_heads, cap, D), got {tuple(q.shape)}, {tuple(k_prefix.shape)}, {tuple(k_tail.shape)}")
+    bf = torch.bfloat16
+    (rows, heads, D), (kv, P, _), (seqs, _, cap, _) = q.shape, k_prefix.shape, k_tail.shape
+    _expect(what, "q", q, bf)
+    _expect(what, "k_prefix", k_prefix, bf, (kv, P, D))
+    _expect(what, "v_prefix", v_prefix, bf, (kv, P, D))
+    _expect(what, "k_tail", k_tail, bf, (seqs, kv, cap, D))
+    _expect(what, "v_tail", v_tail, bf, (seqs, kv, cap, D))
+    _expect(what, "tail_lens", tail_lens, torch.int32, (seqs,), True)
+    if row_starts is not None:
+        _expect(what, "row_starts", row_starts, torch.int32, (seqs + 1,), True)
+    if out is None:
+        out = torch.empty((rows, heads, D), dtype=bf, device=dev)
+    else:
+        _expect(what, "out", out, bf, (rows, heads, D))
+    if D not in (64, 128) or kv < 1 or heads < 1 or heads % kv or (rows and not seqs) or (row_starts is None and seqs and rows % seqs) or max_rows < 0:
+        raise IsstError(f"{what}: {rows} rows of {seqs} sequences, {heads} heads on {kv} key heads of {D} (max_rows {max_rows}) are not supported")
+    a = _PrefixAttn(q.data_ptr(), k_prefix.data_ptr(), v_prefix.data_ptr(), k_tail.data_ptr(), v_tail.data_ptr(), tail_lens.data_ptr(),
+                    None if row_starts is None else row_starts.data_ptr(), out.data_ptr(), *_row_strides(what, "q", q), *_row_strides(what, "out", out),
+                    *_row_strides(what, "k_prefix", k_prefix), *_row_strides(what, "v_prefix", v_prefix), *_row_strides(what, "k_tail", k_tail),
+                    *_row_strides(what, "v_tail", v_tail), rows, seqs, max_rows, heads, kv, D, P, cap, D ** -0.5 if scale is None else scale)
+    ref = C.byref(a)
+    _launch(what, dev, lib.isst_op_prefix_attention_workspace(ref), lambda ws, n, st: lib.isst_op_prefix_attention(ref, ws, n, st))
+    return out
+
+
+def op_gemm_lora(x: torch.Tensor, packed: torch.Tensor, N: int, down: torch.Tensor, up: torch.Tensor, scales: torch.Tensor, row_adapter: torch.Tensor,
+                 out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """bf16(x W^T + scales[a] (x down[a]^T) up[a]^T) with a = row_adapter[m] per row (int32; outside 0 .. n - 1: no adapter).  x (M, K) bf16, packed = op_pack_weight(W (N, K)),
+    down (n, rank, K), up (n, N, rank) bf16, scales (n,) fp32; rank a multiple of 8 up to 128 (pad smaller ones with zeros), K a multiple of 32."""
+    what = "op_gemm_lora"
+    lib = load_library()
+    dev = _on_device(what, x, packed=packed, down=down, up=up, scales=scales, row_adapter=row_adapter, out=out)
+    if x.dim() != 2 or down.dim() != 3:
+        raise IsstError(f"{what}: x (M, K), down (n, rank, K), got {tuple(x.shape)}, {tuple(down.shape)}")
+    bf = torch.bfloat16
+    (M, K), (n, rank, _) = x.shape, down.shape
+    _expect(what, "x", x, bf)
+    _expect(what, "packed", packed, bf, (lib.isst_op_packed_elems(N, K),), True)
+    _expect(what, "down", down, bf, (n, rank, K), True)
+    _expect(what, "up", up, bf, (n, N, rank), True)
+    _expect(what, "scales", scales, torch.float32, (n,), True)
+    _expect(what, "row_adapter", row_adapter, torch.int32, (M,), True)
+    if out is None:
+        out = torch.empty((M, N), dtype=bf, device=dev)
+    else:
+        _expect(what, "out", out, bf, (M, N))
+        if (N > 1 and out.stride(1) != 1) or (M > 1 and out.stride(0) < N):
+            raise IsstError(f"{what}: rows of out must be contiguous and apart (strides {out.stride()})")
+    (lda,) = _row_strides(what, "x", x)
+    if M > 1 and lda < K:
+        raise IsstError(f"{what}: rows of x overlap (strides {x.stride()})")
+    _launch(what, dev, lib.isst_op_gemm_lora_workspace(M, N, K, rank, n),
+            lambda ws, nb, st: lib.isst_op_gemm_lora(x.data_ptr(), lda if M > 1 else K, packed.data_ptr(), down.data_ptr(), up.data_ptr(), scales.data_ptr(),
+                                                     row_adapter.data_ptr(), n, rank, out.data_ptr(), out.stride(0) if M > 1 else N, M, N, K, ws, nb, st))
+    return out
+
+
+def op_verify_drafts(target: torch.Tensor, drafts: torch.Tensor, n_drafts: Optional[torch.Tensor] = None, draft_scores: Optional[torch.Tensor] = None,
+                     uniforms: Optional[torch.Tensor] = None):
+    """Drafted tokens against the model's scores: target (streams, K + 1, vocab) fp32 processed scores (-inf = removed), drafts (streams, K) int32 of which n_drafts[b] (None: all)
+    are live, draft_scores (streams, K, vocab) fp32 or None (a draft without a distribution), uniforms (streams, K + 1) float64 in [0, 1) -- [:, i] decides draft i, [:, K] draws the
+    token behind the last accepted one -- or None: greedy.  Returns (tokens (streams, K + 1) int32: accepted drafts, next token, -1 behind them; counts (streams,) int32, -1 for a
+    stream whose deciding row has no distribution or whose inputs are out of range)."""
+    what = "op_verify_drafts"
+    lib = load_library()
+    dev = _on_device(what, target, drafts=drafts, n_drafts=n_drafts, draft_scores=draft_scores, uniforms=uniforms)
+    if target.dim() != 3 or target.shape[1] < 1 or target.shape[2] < 1:
+        raise IsstError(f"{what}: target (streams, K + 1, vocab), got {tuple(target.shape)}")
+    B, K, V = target.shape[0], target.shape[1] - 1, target.shape[2]
+    _expect(what, "target", target, torch.float32)
+    _expect(what, "drafts", drafts, torch.int32, (B, K), True)
+    if n_drafts is not None:
+        _expect(what, "n_drafts", n_drafts, torch.int32, (B,), True)
+    if draft_scores is not None:
+        _expect(what, "draft_scores", draft_scores, torch.float32, (B, K, V))
+    if uniforms is not None:
+        _expect(what, "uniforms", uniforms, torch.float64, (B, K + 1), True)
+    if uniforms is None and draft_scores is not None:
+        raise IsstError(f"{what}: greedy verification reads no draft scores")
+    for name, t in (("target", target), ("draft_scores", draft_scores)):
+        if t is not None and V > 1 and t.stride(2) != 1:
+            raise IsstError(f"{what}: rows of {name} must be contiguous (strides {t.stride()})")
+    tokens = torch.empty((B, K + 1), dtype=torch.int32, device=dev)
+    counts = torch.empty((B,), dtype=torch.int32, device=dev)
+    ds = (None, 0, 0) if draft_scores is None else (draft_scores.data_ptr(), draft_scores.stride(0), draft_scores.stride(1))
+    _launch(what, dev, lib.isst_op_verify_drafts_workspace(B, K, V),
+            lambda ws, n, st: lib.isst_op_verify_drafts(target.data_ptr(), target.stride(0), target.stride(1), *ds, drafts.data_ptr(), _ptr(n_drafts), _ptr(uniforms), B, K, V,
+                                                        tokens.data_ptr(), counts.data_ptr(), ws, n, st))
+    return tokens, counts
