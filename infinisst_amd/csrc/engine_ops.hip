@@ -273,6 +273,8 @@ static bool prefix_attention_ok(const isst_prefix_attn* a) {
         strides |= a->kt_seq | a->kt_head | a->kt_key | a->vt_seq | a->vt_head | a->vt_key;
     }
     if (strides & 7) return false;
+    for (const int64_t key : {a->kp_key, a->vp_key, a->kt_key, a->vt_key})  // (32-bit offsets inside a tile of 64 keys)
+        if (key < 0 || key > (1 << 24)) return false;
     // two outputs never share memory
     return (a->heads == 1 || a->out_head >= a->head_dim) && (a->rows == 1 || a->out_row >= (a->heads - 1) * a->out_head + a->head_dim);
 }
