@@ -259,7 +259,7 @@ static bool prefix_attention_ok(const isst_prefix_attn* a) {
     if (!a || a->rows < 0 || a->seqs < 0 || a->max_rows < 0 || a->heads < 1 || a->kv_heads < 1 || a->heads % a->kv_heads || (a->head_dim != 64 && a->head_dim != 128) ||
         a->prefix_len < 0 || a->tail_cap < 0 || !(a->scale > 0.f) || !(a->scale < INFINITY))
         return false;
-    if ((int64_t)a->rows * a->heads > (1 << 30) || (a->rows > 0 && a->seqs < 1)) return false;
+    if (a->heads > (1 << 15) || (int64_t)a->rows * a->heads > (1 << 30) || (int64_t)a->seqs * a->kv_heads > (1 << 24) || (a->rows > 0 && a->seqs < 1)) return false;
     if (!a->row_starts && a->seqs > 0 && a->rows % a->seqs) return false;
     if (a->rows == 0) return true;
     if (!a->q || !a->out || !a->tail_lens || !aligned16(a->q) || !aligned16(a->out)) return false;

@@ -11,10 +11,12 @@
 #include "common.h"
 #include "kernels.h"
 
+#include <type_traits>
+
 typedef __attribute__((ext_vector_type(16))) float f32x16_t;
 typedef __attribute__((ext_vector_type(4))) short s16x4_t;
 
-#define PA_TILE 64               // keys of a block tile
+#define PA_TILE 32               // keys of a block tile
 // Keys and values are read through buffer descriptors that start at a tile's first row: a lane's offset is either its row's (rows lie up to 2^25 bytes apart, 63 of them stay inside the
 // descriptor) or PA_OOB, for which the load returns zeros -- also with the scalar offset of the row group added.
 #define PA_EXTENT 0x7fffffffu
@@ -42,12 +44,24 @@ __device__ __forceinline__ int seq_of_row(const isst_prefix_attn& a, int row) {
 }
 
 struct PrefixPlan {
-    int col_tiles, prefix_splits, split_tiles;  // block form: column tiles, key spans of split_tiles tiles.  col_tiles = 0: the prefix runs in span form
-    int own_tiles, own_splits;                  // span form of the own keys: column tiles of a sequence (a longer one walks on), key splits
-    int prefix_units, own_units, slots;
-    float* o;                                   // [slots][rows * heads][D] fp32, unnormalised
-    float2* ml;                                 // [slots][rows * heads]: maximum (in units of log2), sum
+    unsigned magic;                              // ceil(2^32 / G), 0 for G = 1 (group_of)
+    int prefix_block, prefix_tiles, prefix_splits, prefix_units;  // block form or span form; column tiles, key spans; units padded to a multiple of 8
+    int own_block, own_tiles, own_splits, own_units;                           // column tiles of a sequence (a longer one walks on), key spans
+    int slots;
+    float* o;                                    // [slots][rows * heads][D] fp32, unnormalised
+    float2* ml;                                  // [slots][rows * heads]: maximum (in units of log2), sum
 };
+// x / G for a column counted from the start of a row (x < G + 128, G < 2^15: exact)
+__device__ __forceinline__ int group_of(int x, unsigned magic) { return magic ? (int)__umulhi((unsigned)x, magic) : x; }
+// what a workgroup attends to: columns c0 .. ncols - 1 of a sequence (column c = its row c / G, head kvh G + c % G) over `keys` keys; column c sees keys j < limit0 + c / G where causal
+struct KeySpan {
+    const bf16_t *k, *v;
+    long kstride, vstride;
+    int keys, first, ncols, kvh;
+    bool causal;
+    int limit0;
+};
+__device__ __forceinline__ int sees(const KeySpan& s, int t) { return s.causal ? min(max(s.limit0 + t, 0), s.keys) : s.keys; }
 
 // XOR swizzle of the 16-byte chunks of a K / V tile row: 16 rows read at one chunk (K fragments) and 4 rows x 4 chunks (transposed V reads) both cover all 64 banks once
 template <int D>
@@ -62,155 +76,247 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t key_rsrc(const bf16_t* p) {
     return __builtin_amdgcn_make_buffer_rsrc(const_cast<bf16_t*>(p), 0, PA_EXTENT, 0x00020000);
 }
 
+// Keys [lo, hi) of one column added to its stored partial result, whose maximum covers them.  Only for tiles that hold inf or NaN values and that some column of a wave does not see
+// whole: in a matrix product 0 x inf would reach the columns that do not see the key.
+template <int D>
+__device__ void add_keys(const isst_prefix_attn& a, const PrefixPlan& p, const KeySpan& w, int slot, int c, int lo, int hi) {
+    const int G = a.heads / a.kv_heads, t = c / G, head = w.kvh * G + c % G;
+    int lane = threadIdx.x & 63;
+    asm volatile("" : "+v"(lane));
+    const long at = (long)slot * a.rows * a.heads + (long)(w.first + t) * a.heads + head;
+    const float m = p.ml[at].x, neg = m == -INFINITY ? 0.f : -m;
+    const bf16_t* q = a.q + (w.first + t) * a.q_row + head * a.q_head;
+    hi = min(hi, sees(w, t));
+    for (int j = lo; j < hi; ++j) {
+        float s = 0.f;
+        for (int d = lane; d < D; d += 64) s += bf2f(q[d]) * bf2f(w.k[j * w.kstride + d]);
+        const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(wave_sum(s), a.scale * 1.44269504088896340736f, neg));
+        for (int d = lane; d < D; d += 64) p.o[at * D + d] += e * bf2f(w.v[j * w.vstride + d]);
+    }
+}
+
 // ---------------------------------------------------------------------------------------------------------------- block role
+// columns [c0, c0 + 32 NW) against the key tiles of span `split` of `splits`.  A wave owns 32 columns.  K and V tiles go from registers into a ring of three LDS stages; the score product of
+// the next tile is issued with this tile's exponentials, so that the matrix pipe and the vector ALU work at the same time (two workgroups per CU: 256 registers a lane).
 template <int D, int NW>
-__device__ __forceinline__ void block_role(const isst_prefix_attn& a, const PrefixPlan& p, int unit, char* lds) {
-    constexpr int ROWB = 2 * D, CH = D / 8, LOADS = PA_TILE * CH / (NW * 64), RSTEP = NW * 64 / CH, QS = D / 16, DT = D / 32;
+__device__ __forceinline__ void block_role(const isst_prefix_attn& a, const PrefixPlan& p, char* lds, const KeySpan& w, int c0, int split, int splits, int slot) {
+    constexpr int ROWB = 2 * D, CH = D / 8, LOADS = PA_TILE * CH / (NW * 64), RSTEP = NW * 64 / CH, QS = D / 16, DT = D / 32, STAGE = 2 * PA_TILE * ROWB;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), c32 = lane & 31, half = lane >> 5;
-    const int split = unit % p.prefix_splits, ct = (unit / p.prefix_splits) % p.col_tiles, kvh = unit / p.prefix_splits / p.col_tiles;
-    const int G = a.heads / a.kv_heads, cols = a.rows * G;
-    const int tile0 = split * p.split_tiles, tiles = min(p.split_tiles, (a.prefix_len + PA_TILE - 1) / PA_TILE - tile0);
-    const int col = (ct * NW + wave) * 32 + c32;
-    const bool live = col < cols, wave_live = (ct * NW + wave) * 32 < cols;
-    const int row = live ? col / G : 0, head = kvh * G + (live ? col % G : 0);
+    const int G = a.heads / a.kv_heads, cw = c0 + 32 * wave;
+    const int total = (sees(w, (min(c0 + 32 * NW, w.ncols) - 1) / G) + PA_TILE - 1) / PA_TILE, per = (total + splits - 1) / splits, tile0 = split * per, tiles = min(per, total - tile0);
+    const bool wave_live = cw < w.ncols, live = cw + c32 < w.ncols;
+    const int t0 = cw / G, x = cw % G + c32, t = live ? t0 + group_of(x, p.magic) : t0;
+    const int head = w.kvh * G + (live ? x - (t - t0) * G : 0);
+    const int limit = live ? sees(w, t) : w.keys, see_least = sees(w, t0), see_most = wave_live ? sees(w, (min(cw + 32, w.ncols) - 1) / G) : 0;
+    const int mine = min(tiles, (see_most + PA_TILE - 1) / PA_TILE - tile0);  // tiles that this wave's columns see
 
-    u32x4_t qf[QS];
-#pragma unroll
-    for (int s = 0; s < QS; ++s) qf[s] = live ? *reinterpret_cast<const u32x4_t*>(a.q + row * a.q_row + head * a.q_head + 16 * s + 8 * half) : (u32x4_t){0u, 0u, 0u, 0u};
-
-    const bf16_t *kb = a.k_prefix + kvh * a.kp_head, *vb = a.v_prefix + kvh * a.vp_head;
-    const int lr = tid / CH, lc = tid % CH, kstep = (int)a.kp_key * 2, vstep = (int)a.vp_key * 2;
+    const int lr = tid / CH, lc = tid % CH, kstep = (int)w.kstride * 2, vstep = (int)w.vstride * 2;
     const unsigned koff = lr * kstep + lc * 16, voff = lr * vstep + lc * 16;
     u32x4_t ks[LOADS], vs[LOADS];
-    auto fetch = [&](int t) {
-        const int j0 = (tile0 + t) * PA_TILE, rows = min(PA_TILE, a.prefix_len - j0);
-        const __amdgpu_buffer_rsrc_t kr = key_rsrc(kb + j0 * a.kp_key), vr = key_rsrc(vb + j0 * a.vp_key);
+    auto fetch = [&](int i0) {
+        const int j0 = (tile0 + i0) * PA_TILE, rows = w.keys - j0;
+        const __amdgpu_buffer_rsrc_t kr = key_rsrc(w.k + j0 * w.kstride), vr = key_rsrc(w.v + j0 * w.vstride);
 #pragma unroll
         for (int i = 0; i < LOADS; ++i) {
             ks[i] = __builtin_amdgcn_raw_buffer_load_b128(kr, lr < rows - i * RSTEP ? koff : PA_OOB, i * RSTEP * kstep, 0);
             vs[i] = __builtin_amdgcn_raw_buffer_load_b128(vr, lr < rows - i * RSTEP ? voff : PA_OOB, i * RSTEP * vstep, 0);
         }
     };
-    auto put = [&](int buf) {
-        char* base = lds + buf * (2 * PA_TILE * ROWB);
+    auto put = [&](char* base) {
 #pragma unroll
         for (int i = 0; i < LOADS; ++i) {
             *reinterpret_cast<u32x4_t*>(base + tile_off<D>(lr + i * RSTEP, lc)) = ks[i];
             *reinterpret_cast<u32x4_t*>(base + PA_TILE * ROWB + tile_off<D>(lr + i * RSTEP, lc)) = vs[i];
         }
     };
+    if (tiles > 0) fetch(0);
+    u32x4_t qf[QS];
+#pragma unroll
+    for (int s = 0; s < QS; ++s)
+        qf[s] = live ? *reinterpret_cast<const u32x4_t*>(a.q + (w.first + t) * a.q_row + head * a.q_head + 16 * s + 8 * half) : (u32x4_t){0u, 0u, 0u, 0u};
     f32x16_t o[DT];
 #pragma unroll
     for (int d = 0; d < DT; ++d)
 #pragma unroll
         for (int r = 0; r < 16; ++r) o[d][r] = 0.f;
     float m = -INFINITY, l = 0.f;
+    unsigned ill_tiles = 0;
     const float c2 = a.scale * 1.44269504088896340736f;  // exp(scale s - ..) = exp2(c2 s - ..)
 
-    fetch(0);
-    put(0);
+    char *cur = lds, *next = lds + STAGE, *spare = lds + 2 * STAGE;
+    if (tiles > 0) put(cur);
+    if (tiles > 1) { fetch(1); put(next); }
+    if (tiles > 2) fetch(2);
     __syncthreads();
-    for (int t = 0; t < tiles; ++t) {
-        if (t + 1 < tiles) fetch(t + 1);
-        const char* kt = lds + (t & 1) * (2 * PA_TILE * ROWB);
-        const char* vt = kt + PA_TILE * ROWB;
-        if (wave_live) {
-            f32x16_t sc[2];
 #pragma unroll
-            for (int u = 0; u < 2; ++u) {
+    for (int s = 0; s < QS; ++s) asm volatile("" : "+v"(qf[s]));  // (the queries have landed: a wait for them inside the loop would wait for the newest tile as well)
+    auto scores = [&](const char* kt) {
+        f32x16_t sc;
 #pragma unroll
-                for (int r = 0; r < 16; ++r) sc[u][r] = 0.f;
+        for (int r = 0; r < 16; ++r) sc[r] = 0.f;
 #pragma unroll
-                for (int s = 0; s < QS; ++s) {
-                    const u32x4_t kf = *reinterpret_cast<const u32x4_t*>(kt + tile_off<D>(32 * u + c32, 2 * s + half));
-                    sc[u] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8_t, kf), __builtin_bit_cast(bf16x8_t, qf[s]), sc[u], 0, 0, 0);
-                }
+        for (int s = 0; s < QS; ++s) {
+            const u32x4_t kf = *reinterpret_cast<const u32x4_t*>(kt + tile_off<D>(c32, 2 * s + half));
+            sc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8_t, kf), __builtin_bit_cast(bf16x8_t, qf[s]), sc, 0, 0, 0);
+        }
+        return sc;
+    };
+    f32x16_t sc = scores(cur);  // (no tile: of whatever the stage holds, unused -- as behind the last tile below)
+    auto stage = [&](int i) {
+        if (i + 2 < tiles) put(spare);
+        if (i + 3 < tiles) fetch(i + 3);
+    };
+    auto turn = [&]() {
+        __syncthreads();
+        char* done = cur;
+        cur = next; next = spare; spare = done;
+    };
+    // one tile: its scores are in sc, those of the next are computed on the way.  EDGE: some column does not see some key of it
+    auto step = [&](int i, auto edge) {
+        constexpr bool EDGE = decltype(edge)::value;
+        stage(i);
+        const char* vt = cur + PA_TILE * ROWB;
+        const int j0 = (tile0 + i) * PA_TILE;
+        if constexpr (EDGE) {
+            const int lim = limit - j0 - 4 * half;
+#pragma unroll
+            for (int r = 0; r < 16; ++r)
+                if ((r & 3) + 8 * (r >> 2) >= lim) sc[r] = -INFINITY;
+        }
+        float mx = sc[0];
+#pragma unroll
+        for (int r = 1; r < 16; ++r) mx = fmaxf(mx, sc[r]);
+        mx = fmaxf(mx, __shfl_xor(mx, 32, WAVE)) * c2;
+        if (__any(mx > m)) {
+            const float m2 = fmaxf(m, mx), keep = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - m2);
+            l *= keep;
+#pragma unroll
+            for (int d = 0; d < DT; ++d)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) o[d][r] *= keep;
+            m = m2;
+        }
+        const float neg = m == -INFINITY ? 0.f : -m;
+        bool ill = false;  // inf or NaN among the values
+        if constexpr (EDGE) {
+#pragma unroll 1
+            for (int k = 0; k < PA_TILE * ROWB / 1024; ++k) {
+                const u32x4_t v = *reinterpret_cast<const u32x4_t*>(vt + 1024 * k + 16 * lane);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) ill |= (v[e] & 0x7f80u) == 0x7f80u || (v[e] & 0x7f800000u) == 0x7f800000u;
             }
-            const int rows = a.prefix_len - (tile0 + t) * PA_TILE;
-            if (rows < PA_TILE) {  // the prefix ends inside this tile
+            ill = __any(ill);
+        }
+        const f32x16_t sn = scores(next);
+        u32x4_t pf[2];
+        float e[16];
 #pragma unroll
-                for (int u = 0; u < 2; ++u)
+        for (int r = 0; r < 16; ++r) {
+            e[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[r], c2, neg));
+            l += e[r];
+        }
 #pragma unroll
-                    for (int r = 0; r < 16; ++r)
-                        if (32 * u + (r & 3) + 8 * (r >> 2) + 4 * half >= rows) sc[u][r] = -INFINITY;
-            }
-            float mx = -INFINITY;
+        for (int k = 0; k < 2; ++k)
+            pf[k] = (u32x4_t){pack_bf(e[8 * k], e[8 * k + 1]), pack_bf(e[8 * k + 2], e[8 * k + 3]), pack_bf(e[8 * k + 4], e[8 * k + 5]), pack_bf(e[8 * k + 6], e[8 * k + 7])};
+        if (!EDGE || !ill) {
 #pragma unroll
-            for (int u = 0; u < 2; ++u)
+            for (int k = 0; k < 2; ++k)  // 16 keys: slots j < 4 of half h = keys 16 k + 4 h + j, j >= 4 = keys 16 k + 8 + 4 h + (j - 4)
 #pragma unroll
-                for (int r = 0; r < 16; ++r) mx = fmaxf(mx, sc[u][r]);
-            mx = fmaxf(mx, __shfl_xor(mx, 32, WAVE)) * c2;
-            if (__any(mx > m)) {
-                const float m2 = fmaxf(m, mx), keep = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - m2);
-                l *= keep;
-#pragma unroll
-                for (int d = 0; d < DT; ++d)
-#pragma unroll
-                    for (int r = 0; r < 16; ++r) o[d][r] *= keep;
-                m = m2;
-            }
-            const float neg = m == -INFINITY ? 0.f : -m;
-            u32x4_t pf[4];
-#pragma unroll
-            for (int u = 0; u < 2; ++u) {
-                float e[16];
-#pragma unroll
-                for (int r = 0; r < 16; ++r) {
-                    e[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[u][r], c2, neg));
-                    l += e[r];
-                }
-#pragma unroll
-                for (int kb2 = 0; kb2 < 2; ++kb2)
-                    pf[2 * u + kb2] = (u32x4_t){pack_bf(e[8 * kb2], e[8 * kb2 + 1]), pack_bf(e[8 * kb2 + 2], e[8 * kb2 + 3]), pack_bf(e[8 * kb2 + 4], e[8 * kb2 + 5]), pack_bf(e[8 * kb2 + 6], e[8 * kb2 + 7])};
-            }
-#pragma unroll
-            for (int d = 0; d < DT; ++d) {
-                const int ch = 4 * d + 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1);
-#pragma unroll
-                for (int k = 0; k < 4; ++k) {  // 16 keys: slots j < 4 of half h = keys 16 k + 4 h + j, j >= 4 = keys 16 k + 8 + 4 h + (j - 4)
-                    const int r = 16 * k + 4 * half + ((lane >> 2) & 3);
+                for (int d = 0; d < DT; ++d) {
+                    const int ch = 4 * d + 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1), r = 16 * k + 4 * half + ((lane >> 2) & 3);
                     const u32x2_t v1 = read_tr(vt + tile_off<D>(r, ch) + 8 * (lane & 1)), v2 = read_tr(vt + tile_off<D>(r + 8, ch) + 8 * (lane & 1));
                     const u32x4_t vf = {v1.x, v1.y, v2.x, v2.y};
                     o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8_t, vf), __builtin_bit_cast(bf16x8_t, pf[k]), o[d], 0, 0, 0);
                 }
-            }
+        } else {  // the tile's values are added behind the loop
+            ill_tiles |= 1u << min((tile0 + i) - see_least / PA_TILE, 31);
         }
-        if (t + 1 < tiles) put((t + 1) & 1);
-        __syncthreads();
-    }
-    if (!live) return;
+        sc = sn;
+        turn();
+    };
+    const int whole = min(mine, see_least / PA_TILE - tile0);  // tiles that every column of the wave sees whole
+    int i = 0;
+    for (; i < whole; ++i) step(i, std::integral_constant<bool, false>{});
+    for (; i < mine; ++i) step(i, std::integral_constant<bool, true>{});
+    for (; i < tiles; ++i) { stage(i); turn(); }
+    // ---- (m, l) and the accumulators; these turn through the wave's part of LDS so that whole rows of D floats are stored ----
+    int jl = lane;
+    asm volatile("" : "+v"(jl));
     l += __shfl_xor(l, 32, WAVE);
-    const long at = (long)split * a.rows * a.heads + (long)row * a.heads + head;
-    if (half == 0) p.ml[at] = make_float2(m, l);
+    const long base = (long)slot * a.rows * a.heads;
+    if (live && half == 0) p.ml[base + (long)(w.first + t) * a.heads + head] = make_float2(m, l);
+    if (tiles <= 0 || !wave_live) return;  // (uniform per wave; l = 0 tells the join that there is nothing to read)
+    float* red = reinterpret_cast<float*>(lds) + wave * (32 * D);
 #pragma unroll
     for (int d = 0; d < DT; ++d)
 #pragma unroll
-        for (int r4 = 0; r4 < 4; ++r4)
-            *reinterpret_cast<f32x4_t*>(p.o + at * D + 32 * d + 8 * r4 + 4 * half) = (f32x4_t){o[d][4 * r4], o[d][4 * r4 + 1], o[d][4 * r4 + 2], o[d][4 * r4 + 3]};
+        for (int r4 = 0; r4 < 4; ++r4) {
+            const int d4 = 8 * d + 2 * r4 + (jl >> 5), c = jl & 31;
+            *reinterpret_cast<f32x4_t*>(red + c * D + 4 * (d4 ^ (c & (D / 4 - 1)))) = (f32x4_t){o[d][4 * r4], o[d][4 * r4 + 1], o[d][4 * r4 + 2], o[d][4 * r4 + 3]};
+        }
+    __builtin_amdgcn_wave_barrier();
+    constexpr int L4 = D / 4, CPI = 64 / L4;
+    const int d4 = jl % L4;
+    for (int c = jl / L4; c < 32; c += CPI) {
+        if (cw + c >= w.ncols) break;
+        const int xc = cw % G + c, tc = group_of(xc, p.magic);
+        const long at = base + (long)(w.first + t0 + tc) * a.heads + w.kvh * G + (xc - tc * G);
+        *reinterpret_cast<f32x4_t*>(p.o + at * D + 4 * d4) = *reinterpret_cast<const f32x4_t*>(red + c * D + 4 * (d4 ^ (c & (L4 - 1))));
+    }
+    if (ill_tiles) {
+        __threadfence_block();
+        for (int c = 0; c < 32 && cw + c < w.ncols; ++c)
+            for (int k = 0; k < 32; ++k)
+                if (ill_tiles >> k & 1) {
+                    const int j = (see_least / PA_TILE + k) * PA_TILE;
+                    add_keys<D>(a, p, w, slot, cw + c, j, j + PA_TILE);
+                }
+    }
 }
 
 // ---------------------------------------------------------------------------------------------------------------- span role
-// keys 0 .. see(last column) of (kb, vb) for columns [c0, c0 + 16 NQ) of `ncols` (column c = row first + c / G, head kvh G + c % G); column c sees keys j < limit0 + c / G (limit0 < 0: all `keys`)
+// columns [c0, c0 + 16 NQ) over all their keys; the waves of `splits` workgroups take 32 keys at a time each and are joined at the end
 template <int D, int NW, int NQ>
-__device__ __forceinline__ void span_role(const isst_prefix_attn& a, const PrefixPlan& p, char* lds, int kvh, int first, int c0, int ncols, const bf16_t* kb, long kstride, const bf16_t* vb,
-                                          long vstride, int keys, bool causal, int limit0, int split, int splits, int slot) {
+__device__ __forceinline__ void span_role(const isst_prefix_attn& a, const PrefixPlan& p, char* lds, const KeySpan& w, int c0, int split, int splits, int slot) {
     constexpr int ROWB = 2 * D, CH = D / 8, VL = 32 * CH / 64, VR = 64 / CH, QS = D / 32, NT = D / 16;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), fr = lane & 15, fq = lane >> 4;
-    const int G = a.heads / a.kv_heads;
+    const int G = a.heads / a.kv_heads, t0 = c0 / G, x0 = c0 % G;
+    const int see_least = sees(w, t0), see_most = sees(w, (min(c0 + 16 * NQ, w.ncols) - 1) / G);
+    char* vl = lds + wave * (32 * ROWB);
+    u32x4_t kf[2][QS], vr[VL];
+    const int kstep = (int)w.kstride * 2, vstep = (int)w.vstride * 2;
+    const unsigned koff = fr * kstep + 16 * fq, voff = lane / CH * vstep + 16 * (lane % CH);
+    auto fetch_k = [&](int j0) {
+        const __amdgpu_buffer_rsrc_t r = key_rsrc(w.k + j0 * w.kstride);
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+            const unsigned off = fr < see_most - j0 - 16 * t ? koff : PA_OOB;
+#pragma unroll
+            for (int s = 0; s < QS; ++s) kf[t][s] = __builtin_amdgcn_raw_buffer_load_b128(r, off, 16 * t * kstep + 64 * s, 0);
+        }
+    };
+    auto fetch_v = [&](int j0) {
+        const __amdgpu_buffer_rsrc_t r = key_rsrc(w.v + j0 * w.vstride);
+#pragma unroll
+        for (int i = 0; i < VL; ++i) vr[i] = __builtin_amdgcn_raw_buffer_load_b128(r, lane / CH < see_most - j0 - i * VR ? voff : PA_OOB, i * VR * vstep, 0);
+    };
+    __shared__ unsigned ill_steps;
+    if (tid == 0) ill_steps = 0;
+    __syncthreads();
+    const int step = 32 * NW * splits;
+    int j0 = 32 * (split * NW + wave);
+    if (j0 < see_most) { fetch_v(j0); fetch_k(j0); }
+
     int limit[NQ];
     u32x4_t qf[NQ][QS];
 #pragma unroll
     for (int n = 0; n < NQ; ++n) {
-        const int c = c0 + 16 * n + fr;
-        const bool live = c < ncols;
-        const int row = first + (live ? c / G : 0), head = kvh * G + (live ? c % G : 0);
-        limit[n] = causal && live ? min(max(limit0 + c / G, 0), keys) : keys;
+        const bool live = c0 + 16 * n + fr < w.ncols;
+        const int x = x0 + 16 * n + fr, tc = live ? group_of(x, p.magic) : 0, row = w.first + t0 + tc, head = w.kvh * G + (live ? x - tc * G : 0);
+        limit[n] = live ? sees(w, t0 + tc) : w.keys;
 #pragma unroll
         for (int s = 0; s < QS; ++s) qf[n][s] = live ? *reinterpret_cast<const u32x4_t*>(a.q + row * a.q_row + head * a.q_head + 32 * s + 8 * fq) : (u32x4_t){0u, 0u, 0u, 0u};
     }
-    const int last = min(c0 + 16 * NQ, ncols) - 1;
-    const int see_least = causal ? min(max(limit0 + c0 / G, 0), keys) : keys, see_most = causal ? min(max(limit0 + last / G, 0), keys) : keys;
-
     f32x4_t o[NQ][NT];
     float m[NQ], l[NQ];
 #pragma unroll
@@ -220,27 +326,6 @@ __device__ __forceinline__ void span_role(const isst_prefix_attn& a, const Prefi
         for (int t = 0; t < NT; ++t) o[n][t] = (f32x4_t){0.f, 0.f, 0.f, 0.f};
     }
     const float c2 = a.scale * 1.44269504088896340736f;
-    char* vl = lds + wave * (32 * ROWB);
-    u32x4_t kf[2][QS], vr[VL];
-    const int kstep = (int)kstride * 2, vstep = (int)vstride * 2;
-    const unsigned koff = fr * kstep + 16 * fq, voff = lane / CH * vstep + 16 * (lane % CH);
-    auto fetch_k = [&](int j0) {
-        const __amdgpu_buffer_rsrc_t r = key_rsrc(kb + j0 * kstride);
-#pragma unroll
-        for (int t = 0; t < 2; ++t) {
-            const unsigned off = fr < see_most - j0 - 16 * t ? koff : PA_OOB;
-#pragma unroll
-            for (int s = 0; s < QS; ++s) kf[t][s] = __builtin_amdgcn_raw_buffer_load_b128(r, off, 16 * t * kstep + 64 * s, 0);
-        }
-    };
-    auto fetch_v = [&](int j0) {
-        const __amdgpu_buffer_rsrc_t r = key_rsrc(vb + j0 * vstride);
-#pragma unroll
-        for (int i = 0; i < VL; ++i) vr[i] = __builtin_amdgcn_raw_buffer_load_b128(r, lane / CH < see_most - j0 - i * VR ? voff : PA_OOB, i * VR * vstep, 0);
-    };
-    const int step = 32 * NW * splits;
-    int j0 = 32 * (split * NW + wave);
-    if (j0 < see_most) { fetch_v(j0); fetch_k(j0); }
     for (; j0 < see_most; j0 += step) {
 #pragma unroll
         for (int i = 0; i < VL; ++i) *reinterpret_cast<u32x4_t*>(vl + tile_off<D>(i * VR + lane / CH, lane % CH)) = vr[i];
@@ -303,39 +388,9 @@ __device__ __forceinline__ void span_role(const isst_prefix_attn& a, const Prefi
 #pragma unroll
                 for (int w = 0; w < 4; ++w) ill |= (v[w] & 0x7f80u) == 0x7f80u || (v[w] & 0x7f800000u) == 0x7f800000u;
             }
-            if (__any(ill)) {
-                // 0 x inf must not reach a column that does not see the key: the keys that every column sees go through the matrix product below, the others (they see_least ..
-                // see_most of this step) are added here where they are seen and their rows cleared
-                int vb = fq;
-                asm volatile("" : "+v"(vb));  // (keeps this block's addresses out of the loop's preheader: they would take the registers of the ordinary path)
-#pragma unroll 1
-                for (int q = 0; q < 4; ++q)
-#pragma unroll
-                    for (int k = 0; k < 8; ++k) {
-                        const int key = 16 * (k >> 2) + 4 * q + (k & 3);
-                        if (j0 + key < see_least) continue;
-                        float pk[NQ];
-#pragma unroll
-                        for (int n = 0; n < NQ; ++n) {
-                            const uint32_t w = (uint32_t)__shfl((int)pf[n][k >> 1], 16 * q + fr, WAVE);
-                            pk[n] = (k & 1) ? hi_bf(w) : lo_bf(w);
-                        }
-#pragma unroll
-                        for (int t = 0; t < NT; ++t) {
-                            const u32x2_t v = *reinterpret_cast<const u32x2_t*>(vl + tile_off<D>(key, 2 * t + (vb >> 1)) + 8 * (vb & 1));
-#pragma unroll
-                            for (int n = 0; n < NQ; ++n)
-                                if (j0 + key < limit[n]) {
-                                    o[n][t][0] += pk[n] * lo_bf(v.x); o[n][t][1] += pk[n] * hi_bf(v.x);
-                                    o[n][t][2] += pk[n] * lo_bf(v.y); o[n][t][3] += pk[n] * hi_bf(v.y);
-                                }
-                        }
-                    }
-                __builtin_amdgcn_wave_barrier();
-#pragma unroll
-                for (int i = 0; i < VL; ++i)
-                    if (j0 + i * VR + lane / CH >= see_least) *reinterpret_cast<u32x4_t*>(vl + tile_off<D>(i * VR + lane / CH, lane % CH) + (vb - fq)) = (u32x4_t){0u, 0u, 0u, 0u};
-                __builtin_amdgcn_wave_barrier();
+            if (__any(ill)) {  // the step's values are added behind the join
+                if (lane == 0) atomicOr(&ill_steps, 1u << min((j0 >> 5) - (see_least >> 5), 31));
+                continue;
             }
         }
         const int vrow = 4 * fq + ((lane >> 2) & 3), vch = (lane & 3) >> 1, vb8 = 8 * (lane & 1);
@@ -381,108 +436,160 @@ __device__ __forceinline__ void span_role(const isst_prefix_attn& a, const Prefi
             f32x4_t s = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
             for (int w = 0; w < NW; ++w) s += *reinterpret_cast<const f32x4_t*>(red + (w * 16 + c) * D + 4 * ((d4 & ~3) | ((d4 ^ c) & 3)));
-            const int cc = c0 + 16 * n + c;
-            if (cc < ncols) {
-                const long at = (long)slot * a.rows * a.heads + (long)(first + cc / G) * a.heads + kvh * G + cc % G;
+            if (c0 + 16 * n + c < w.ncols) {
+                const int x = x0 + 16 * n + c, tc = group_of(x, p.magic);
+                const long at = (long)slot * a.rows * a.heads + (long)(w.first + t0 + tc) * a.heads + w.kvh * G + (x - tc * G);
                 *reinterpret_cast<f32x4_t*>(p.o + at * D + 4 * d4) = s;
             }
         }
-        if (wave == 0 && jq == 0 && c0 + 16 * n + jc < ncols) {
-            const int cc = c0 + 16 * n + jc;
-            p.ml[(long)slot * a.rows * a.heads + (long)(first + cc / G) * a.heads + kvh * G + cc % G] = make_float2(M, L);
+        if (wave == 0 && jq == 0 && c0 + 16 * n + jc < w.ncols) {
+            const int x = x0 + 16 * n + jc, tc = group_of(x, p.magic);
+            p.ml[(long)slot * a.rows * a.heads + (long)(w.first + t0 + tc) * a.heads + w.kvh * G + (x - tc * G)] = make_float2(M, L);
         }
         __syncthreads();
     }
+    if (ill_steps && wave == 0)
+        for (int c = c0; c < min(c0 + 16 * NQ, w.ncols); ++c)
+            for (int k = 0; k < 32; ++k)
+                if (ill_steps >> k & 1) add_keys<D>(a, p, w, slot, c, ((see_least >> 5) + k) * 32, ((see_least >> 5) + k) * 32 + 32);
 }
 
 template <int D, int NW, int NQ>
 __global__ __launch_bounds__(NW * 64, 2) void prefix_attn_partial_kernel(isst_prefix_attn a, PrefixPlan p) {
-    constexpr int BLOCK_LDS = 4 * PA_TILE * 2 * D, SPAN_LDS = NW * 16 * D * 4;
+    constexpr int BLOCK_LDS = 3 * 2 * PA_TILE * 2 * D, SPAN_LDS = NW * 32 * D * 4;  // (ring of three stages; the turned accumulators of a block, the value tiles and the join of a span)
     __shared__ __attribute__((aligned(16))) char lds[BLOCK_LDS > SPAN_LDS ? BLOCK_LDS : SPAN_LDS];
-    int unit = blockIdx.x;
-    const bool prefix = unit < p.prefix_units;
-    if (prefix && p.col_tiles) {
-        block_role<D, NW>(a, p, unit, lds);
-        return;
-    }
-    // span role: of the own keys of a sequence, or of the prefix for a batch of no more than one column tile
-    if (!prefix) unit -= p.prefix_units;
-    const int splits = prefix ? p.prefix_splits : p.own_splits, tiles = prefix ? 1 : p.own_tiles;
-    const int split = unit % splits, ct = unit / splits % tiles, kvh = unit / splits / tiles % a.kv_heads, b = unit / splits / tiles / a.kv_heads, G = a.heads / a.kv_heads;
-    int first = 0, n = a.rows, keys = a.prefix_len, limit0 = a.prefix_len;
-    if (!prefix) {
+    // workgroup i runs on XCD i % 8 (each with an L2 of its own): the column tiles that read the same keys are neighbours on one XCD
+    const bool prefix = (int)blockIdx.x < p.prefix_units;
+    const int unit = prefix ? blockIdx.x : blockIdx.x - p.prefix_units, G = a.heads / a.kv_heads;
+    const int splits = prefix ? p.prefix_splits : p.own_splits, tiles = prefix ? p.prefix_tiles : p.own_tiles;
+    const int ct = (unit >> 3) % tiles, g = (unit >> 3) / tiles * 8 + (unit & 7);
+    const int kvh = g % a.kv_heads, split = g / a.kv_heads % splits, b = g / a.kv_heads / splits;
+    if (b >= (prefix ? 1 : a.seqs)) return;  // (padding)
+    KeySpan w;
+    int n = a.rows;
+    if (prefix) {
+        w = {a.k_prefix + kvh * a.kp_head, a.v_prefix + kvh * a.vp_head, a.kp_key, a.vp_key, a.prefix_len, 0, a.rows * G, kvh, false, 0};
+    } else {
+        int first, len = a.tail_lens[b];
         seq_rows(a, b, first, n);
-        first = __builtin_amdgcn_readfirstlane(first);  // (uniform already; a value the compiler keeps in a vector register would make every key load a loop over lanes)
+        first = __builtin_amdgcn_readfirstlane(first);  // (uniform already; a value that the compiler keeps in a vector register would make every key load a loop over lanes)
         n = __builtin_amdgcn_readfirstlane(n);
-        keys = __builtin_amdgcn_readfirstlane(a.tail_lens[b]);
-        keys = min(max(keys, 0), a.tail_cap);
-        limit0 = keys - n + 1;
+        len = min(max(__builtin_amdgcn_readfirstlane(len), 0), a.tail_cap);
+        w = {a.k_tail + b * a.kt_seq + kvh * a.kt_head, a.v_tail + b * a.vt_seq + kvh * a.vt_head, a.kt_key, a.vt_key, len, first, n * G, kvh, true, len - n + 1};
     }
-    const bf16_t* kb = prefix ? a.k_prefix + kvh * a.kp_head : a.k_tail + b * a.kt_seq + kvh * a.kt_head;
-    const bf16_t* vb = prefix ? a.v_prefix + kvh * a.vp_head : a.v_tail + b * a.vt_seq + kvh * a.vt_head;
-    for (int c0 = ct * 16 * NQ; c0 < n * G; c0 += tiles * 16 * NQ)
-        span_role<D, NW, NQ>(a, p, lds, kvh, first, c0, n * G, kb, prefix ? a.kp_key : a.kt_key, vb, prefix ? a.vp_key : a.vt_key, keys, !prefix, limit0, split, splits,
-                             prefix ? split : p.prefix_splits + split);
+    const bool block = prefix ? p.prefix_block : p.own_block;
+    const int width = block ? 32 * NW : 16 * NQ, slot = prefix ? split : p.prefix_splits + split;
+    for (int c0 = ct * width; c0 < w.ncols; c0 += tiles * width) {
+        if (c0 != ct * width) __syncthreads();  // (LDS is the last tile's until all are done with it)
+        if (block) block_role<D, NW>(a, p, lds, w, c0, split, splits, slot);
+        else span_role<D, NW, NQ>(a, p, lds, w, c0, split, splits, slot);
+    }
 }
 
-// joins the slots of a (row, head): D / 4 lanes each
+// Joins the slots of a (row, head), D / 4 lanes each.  Bound by latency: the statistics of all slots come in one load (lane i: slot i), the accumulators eight slots at a time.
+#define PA_MAX_SLOTS 32
 template <int D>
 __global__ __launch_bounds__(256) void prefix_attn_join_kernel(isst_prefix_attn a, PrefixPlan p) {
-    constexpr int L4 = D / 4;
-    const long pair = (long)blockIdx.x * (256 / L4) + threadIdx.x / L4;
-    const int d4 = threadIdx.x % L4;
-    if (pair >= (long)a.rows * a.heads) return;
+    constexpr int L4 = D / 4, E = PA_MAX_SLOTS / L4;
+    const long pair = (long)blockIdx.x * (256 / L4) + threadIdx.x / L4, stride = (long)a.rows * a.heads;
+    const int i = threadIdx.x % L4;
+    if (pair >= stride) return;
     const int row = (int)(pair / a.heads), head = (int)(pair % a.heads);
+    float m[E], w[E], M = -INFINITY, L = 0.f;
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+        const int s = i + e * L4;
+        const float2 x = s < p.slots ? p.ml[s * stride + pair] : make_float2(-INFINITY, 0.f);
+        m[e] = x.x; w[e] = x.y;
+        M = fmaxf(M, x.x);
+    }
     if (seq_of_row(a, row) < 0) return;
-    const long stride = (long)a.rows * a.heads;
-    float M = -INFINITY, L = 0.f;
-    for (int s = 0; s < p.slots; ++s) M = fmaxf(M, p.ml[s * stride + pair].x);
+#pragma unroll
+    for (int d = 1; d < L4; d <<= 1) M = fmaxf(M, __shfl_xor(M, d, WAVE));
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+        const float l = w[e];
+        w[e] = l == 0.f ? 0.f : m[e] == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m[e] - M);  // (no key: nothing; -inf with a sum: NaN scores only)
+        L += l == 0.f ? 0.f : l * w[e];
+    }
+#pragma unroll
+    for (int d = 1; d < L4; d <<= 1) L += __shfl_xor(L, d, WAVE);
     f32x4_t o = {0.f, 0.f, 0.f, 0.f};
-    for (int s = 0; s < p.slots; ++s) {
-        const float2 x = p.ml[s * stride + pair];
-        if (x.y == 0.f) continue;  // no key
-        const float w = x.x == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(x.x - M);  // (-inf with a sum: NaN scores only)
-        L += x.y * w;
-        o += *reinterpret_cast<const f32x4_t*>(p.o + (s * stride + pair) * D + 4 * d4) * w;
+    const float* src = p.o + pair * D + 4 * i;
+    for (int s0 = 0; s0 < p.slots; s0 += 8) {
+        f32x4_t x[8];
+        float ws[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+            const int s = s0 + k;
+            ws[k] = s < p.slots ? __shfl(E == 1 || s0 < L4 ? w[0] : w[E - 1], s % L4, L4) : 0.f;
+            x[k] = ws[k] != 0.f ? *reinterpret_cast<const f32x4_t*>(src + s * stride * D) : (f32x4_t){0.f, 0.f, 0.f, 0.f};
+        }
+#pragma unroll
+        for (int k = 0; k < 8; ++k) o += x[k] * ws[k];
     }
     const float inv = L != 0.f ? 1.f / L : 0.f;
     const u32x2_t r = {pack_bf(o.x * inv, o.y * inv), pack_bf(o.z * inv, o.w * inv)};
-    *reinterpret_cast<u32x2_t*>(a.out + row * a.out_row + head * a.out_head + 4 * d4) = r;
+    *reinterpret_cast<u32x2_t*>(a.out + row * a.out_row + head * a.out_head + 4 * i) = r;
 }
 
 // ---------------------------------------------------------------------------------------------------------------- host
-#define PA_NW 8
+#ifndef PA_NW
+#define PA_NW 4
+#endif
+#ifndef PA_TAU
+#define PA_TAU 1.25
+#endif
+#ifndef PA_FIX
+#define PA_FIX 5.0
+#endif
 static int ceil_div(long a, long b) { return (int)((a + b - 1) / b); }
+// most columns of a sequence that the launch is shaped for
+static long own_columns(const isst_prefix_attn& a) {
+    const int rows = a.row_starts ? (a.max_rows ? a.max_rows : ceil_div(a.rows, a.seqs)) : a.rows / a.seqs;
+    return (long)(rows > 0 ? rows : 1) * (a.heads / a.kv_heads);
+}
 static int span_nq(const isst_prefix_attn& a) {
-    const int G = a.heads / a.kv_heads, rows = a.row_starts ? (a.max_rows ? a.max_rows : ceil_div(a.rows, a.seqs)) : a.rows / a.seqs;
-    return (long)rows * G > 16 ? 2 : 1;
+    const long own = a.tail_cap > 0 ? own_columns(a) : 0, all = a.prefix_len > 0 ? (long)a.rows * (a.heads / a.kv_heads) : 0;
+    return (own > 16 && own <= 32) || (all > 16 && all <= 32) ? 2 : 1;
 }
 static PrefixPlan plan(const isst_prefix_attn& a) {
     PrefixPlan p{};
-    const int G = a.heads / a.kv_heads, nq = span_nq(a);
+    const int G = a.heads / a.kv_heads, nq = span_nq(a), width = 32 * PA_NW;
+    p.magic = G > 1 ? (unsigned)(((1ull << 32) + G - 1) / G) : 0;
     const long cols = (long)a.rows * G;
-    if (a.prefix_len > 0) {
-        if (cols <= 16 * nq) {
-            p.prefix_splits = ceil_div(a.prefix_len, 32 * PA_NW);
-            if (p.prefix_splits > 32) p.prefix_splits = 32;
-            p.prefix_units = a.kv_heads * p.prefix_splits;
-        } else {
-            p.col_tiles = ceil_div(cols, 32 * PA_NW);
-            const int tiles = ceil_div(a.prefix_len, PA_TILE), base = a.kv_heads * p.col_tiles;
-            int splits = base >= 256 ? 1 : 256 / base;
-            if (splits > tiles) splits = tiles;
-            p.split_tiles = ceil_div(tiles, splits);
-            p.prefix_splits = ceil_div(tiles, p.split_tiles);
-            p.prefix_units = base * p.prefix_splits;
-        }
-    }
+    const double room = 256.0 * (8 / PA_NW);  // workgroups the chip runs at once
+    double own_us = 0;                        // time of the own keys' units, summed
     if (a.tail_cap > 0) {
-        const int rows = a.row_starts ? (a.max_rows ? a.max_rows : ceil_div(a.rows, a.seqs)) : a.rows / a.seqs;
-        p.own_tiles = ceil_div((long)(rows > 0 ? rows : 1) * G, 16 * nq);
-        const long units = (long)a.seqs * a.kv_heads * p.own_tiles;
+        const long oc = own_columns(a);
+        p.own_block = oc > 32;
+        p.own_tiles = ceil_div(oc, p.own_block ? width : 16 * nq);
+        const long groups = (long)a.seqs * a.kv_heads, keys = p.own_block ? PA_TILE : 32 * PA_NW;
         p.own_splits = 1;
-        while (p.own_splits < 16 && units * p.own_splits * 2 <= 256 && p.own_splits * 2 <= ceil_div(a.tail_cap, 32 * PA_NW)) p.own_splits *= 2;
-        p.own_units = (int)(units * p.own_splits);
+        while (p.own_splits < 8 && groups * p.own_tiles * p.own_splits * 2 <= room && p.own_splits * 2 <= ceil_div(a.tail_cap, (p.own_block ? 4 : 2) * keys)) p.own_splits *= 2;
+        p.own_units = p.own_tiles * 8 * ceil_div(groups * p.own_splits, 8);
+        own_us = (double)groups * p.own_tiles * (p.own_block ? a.tail_cap / 2 / (double)PA_TILE * PA_TAU : a.tail_cap / 2 * (4.0 * a.head_dim) / (20e3 * PA_NW / 8));
+    }
+    if (a.prefix_len > 0) {
+        p.prefix_block = cols > 32;
+        p.prefix_tiles = p.prefix_block ? ceil_div(cols, width) : 1;
+        if (p.prefix_block) {
+            // key spans: the rounds of the chip that the units take (with the own keys' units filling what a last round leaves) + what their partial results cost
+            const int tiles = ceil_div(a.prefix_len, PA_TILE), groups = a.kv_heads * p.prefix_tiles;
+            double best = 1e30;
+            for (int s = 1; s <= PA_MAX_SLOTS - 8 && s <= tiles; ++s) {
+                const int per = ceil_div(tiles, s);
+                if (ceil_div(tiles, per) != s) continue;
+                const double dur = per * PA_TAU * (a.head_dim / 128.0) + PA_FIX, units = (double)groups * s;
+                const double even = (units * dur + own_us) / room, rounds = dur * ceil_div((long)units, (long)room);
+                const double t = (even > rounds ? even : rounds) + s * (double)a.rows * a.heads * (8.0 * a.head_dim) / 3e6;
+                if (t < best) { best = t; p.prefix_splits = s; }
+            }
+        } else {
+            p.prefix_splits = ceil_div(a.prefix_len, 32 * PA_NW);
+            if (p.prefix_splits > PA_MAX_SLOTS - 8) p.prefix_splits = PA_MAX_SLOTS - 8;
+        }
+        p.prefix_units = p.prefix_tiles * 8 * ceil_div((long)a.kv_heads * p.prefix_splits, 8);
     }
     p.slots = p.prefix_splits + p.own_splits;
     return p;
