@@ -333,7 +333,7 @@ extern "C" int isst_op_gemm_lora(const uint16_t* A, int64_t lda, const uint16_t*
 }
 
 static bool verify_ok(int streams, int max_drafts, int vocab) {
-    return streams >= 0 && max_drafts >= 0 && vocab >= 1 && (int64_t)streams * (2 * (int64_t)max_drafts + 1) < (1 << 24);
+    return streams >= 0 && max_drafts >= 0 && max_drafts < (1 << 14) && vocab >= 1 && vocab <= (1 << 30) && streams < (1 << 24);
 }
 extern "C" int64_t isst_op_verify_drafts_workspace(int streams, int max_drafts, int vocab) {
     return verify_ok(streams, max_drafts, vocab) ? verify_workspace(streams, max_drafts, vocab) : ISST_ERR_ARG;
@@ -350,7 +350,7 @@ extern "C" int isst_op_verify_drafts(const float* target, int64_t target_stream,
     if (workspace_bytes < verify_workspace(streams, max_drafts, vocab)) return ISST_ERR_NOMEM;
     VerifyArgs v{};
     v.target = target; v.target_stream = target_stream; v.target_row = target_row;
-    v.draft = max_drafts > 0 ? draft_scores : nullptr; v.draft_stream = draft_stream; v.draft_row = draft_row;
+    v.draft = max_drafts > 0 && uniforms ? draft_scores : nullptr; v.draft_stream = draft_stream; v.draft_row = draft_row;
     v.drafts = drafts; v.n_drafts = n_drafts; v.uniforms = uniforms; v.streams = streams; v.max_drafts = max_drafts; v.vocab = vocab;
     v.tokens = tokens; v.counts = counts; v.workspace = workspace;
     return launch_verify(v, reinterpret_cast<hipStream_t>(hip_stream));
