@@ -737,43 +737,47 @@ def op_llm_attention(qkv: torch.Tensor, pos0: int, kpool: torch.Tensor, krpool: 
 
 
 # ---------------------------------------------------------------- a decode step of many streams over one prompt
-def _on_device(what: str, first: torch.Tensor, **tensors):
-    """Every given tensor lies on `first`'s GPU; returns that device (the ops below run there, on its current stream)."""
-    dev = first.device
-    if dev.type != "cuda":
-        raise IsstError(f"{what}: tensors must be on a GPU, got {dev}")
-    for name, t in tensors.items():
-        if t is not None and t.device != dev:
-            raise IsstError(f"{what}: {name} is on {t.device}, expected {dev}")
-    return dev
+# (these functions cost a decode step some ten microseconds of host time each next to kernels that take as long: their checks are written for the call that passes)
+def _device_of(what: str, t: torch.Tensor) -> int:
+    if t.get_device() < 0 or not t.is_cuda:
+        raise IsstError(f"{what}: tensors must be on a GPU, got {t.device}")
+    return t.get_device()
 
 
-def _expect(what: str, name: str, t: torch.Tensor, dtype: torch.dtype, shape=None, contiguous: bool = False):
-    if t.dtype != dtype or (shape is not None and tuple(t.shape) != tuple(shape)):
-        raise IsstError(f"{what}: {name} must be {dtype}{'' if shape is None else ' ' + str(tuple(shape))}, got {t.dtype} {tuple(t.shape)}")
+def _expect(what: str, dev: int, name: str, t: torch.Tensor, dtype: torch.dtype, shape, contiguous: bool = True):
+    if t.dtype is not dtype or t.shape != shape:
+        raise IsstError(f"{what}: {name} must be {dtype} {tuple(shape)}, got {t.dtype} {tuple(t.shape)}")
+    if t.get_device() != dev:
+        raise IsstError(f"{what}: {name} is on {t.device}, expected cuda:{dev}")
     if contiguous and not t.is_contiguous():
-        raise IsstError(f"{what}: {name} must be contiguous")
+        raise IsstError(f"{what}: {name} must be contiguous (strides {t.stride()})")
 
 
-def _row_strides(what: str, name: str, t: torch.Tensor) -> list:
+def _row_strides(what: str, name: str, t: torch.Tensor):
     """Strides of all dims but the last (0 where a dim has no second entry), for rows the kernels read 16 bytes at a time."""
+    st = t.stride()
+    bits = 0
+    for s in st[:-1]:
+        bits |= s
+    if st[-1] == 1 and not bits & 7 and not t.data_ptr() & 15:
+        return st[:-1]
     if t.numel() == 0:
-        return [0] * (t.dim() - 1)
-    st = [s if n > 1 else 0 for s, n in zip(t.stride()[:-1], t.shape[:-1])]
+        return (0,) * (t.dim() - 1)
+    st = tuple(s if n > 1 else 0 for s, n in zip(t.stride()[:-1], t.shape[:-1]))
     if (t.stride(-1) != 1 and t.shape[-1] > 1) or t.data_ptr() % 16 or any(s % 8 for s in st):
         raise IsstError(f"{what}: rows of {name} must be contiguous and 16-byte aligned (strides {t.stride()})")
     return st
 
 
-def _launch(what: str, dev: torch.device, workspace_bytes: int, call):
-    """call(workspace pointer, bytes, stream) on `dev`'s current stream; the workspace is the caching allocator's, i.e. ordered by that stream."""
+def _launch(what: str, dev: int, workspace_bytes: int, call):
+    """call(workspace pointer, bytes, stream) on the current stream of `dev`; the workspace is the caching allocator's, i.e. ordered by that stream."""
     if workspace_bytes < 0:
         raise IsstError(f"{what}: bad arguments ({workspace_bytes})")
-    if dev.index != torch.cuda.current_device():
+    if dev != torch.cuda.current_device():
         with torch.cuda.device(dev):
             return _launch(what, dev, workspace_bytes, call)
     ws = torch.empty(workspace_bytes, dtype=torch.uint8, device=dev) if workspace_bytes else None
-    rc = call(None if ws is None else ws.data_ptr(), workspace_bytes, torch.cuda.current_stream().cuda_stream)
+    rc = call(None if ws is None else ws.data_ptr(), workspace_bytes, torch._C._cuda_getCurrentRawStream(dev))
     if rc:
         raise IsstError(f"{what} -> {rc}")
 
@@ -786,24 +790,25 @@ def op_prefix_attention(q: torch.Tensor, k_prefix: torch.Tensor, v_prefix: torch
     undefined without).  max_rows: most rows of one sequence if the caller knows it (speed only).  bf16, D 64 or 128, keys already rotated; strided views are fine while
     rows are 16-byte aligned.  scale: default D ** -0.5."""
     what = "op_prefix_attention"
-    lib = load_library()
-    dev = _on_device(what, q, k_prefix=k_prefix, v_prefix=v_prefix, k_tail=k_tail, v_tail=v_tail, tail_lens=tail_lens, row_starts=row_starts, out=out)
+    lib = _lib or load_library()
+    dev = _device_of(what, q)
     if q.dim() != 3 or k_prefix.dim() != 3 or k_tail.dim() != 4:
         raise IsstError(f"{what}: q (rows, heads, D), k_prefix (kv_heads, P, D), k_tail (seqs, kv_heads, cap, D), got {tuple(q.shape)}, {tuple(k_prefix.shape)}, {tuple(k_tail.shape)}")
     bf = torch.bfloat16
     (rows, heads, D), (kv, P, _), (seqs, _, cap, _) = q.shape, k_prefix.shape, k_tail.shape
-    _expect(what, "q", q, bf)
-    _expect(what, "k_prefix", k_prefix, bf, (kv, P, D))
-    _expect(what, "v_prefix", v_prefix, bf, (kv, P, D))
-    _expect(what, "k_tail", k_tail, bf, (seqs, kv, cap, D))
-    _expect(what, "v_tail", v_tail, bf, (seqs, kv, cap, D))
-    _expect(what, "tail_lens", tail_lens, torch.int32, (seqs,), True)
+    prefix, tail = (kv, P, D), (seqs, kv, cap, D)
+    _expect(what, dev, "q", q, bf, (rows, heads, D), False)
+    _expect(what, dev, "k_prefix", k_prefix, bf, prefix, False)
+    _expect(what, dev, "v_prefix", v_prefix, bf, prefix, False)
+    _expect(what, dev, "k_tail", k_tail, bf, tail, False)
+    _expect(what, dev, "v_tail", v_tail, bf, tail, False)
+    _expect(what, dev, "tail_lens", tail_lens, torch.int32, (seqs,))
     if row_starts is not None:
-        _expect(what, "row_starts", row_starts, torch.int32, (seqs + 1,), True)
+        _expect(what, dev, "row_starts", row_starts, torch.int32, (seqs + 1,))
     if out is None:
         out = torch.empty((rows, heads, D), dtype=bf, device=dev)
     else:
-        _expect(what, "out", out, bf, (rows, heads, D))
+        _expect(what, dev, "out", out, bf, (rows, heads, D), False)
     if D not in (64, 128) or kv < 1 or heads < 1 or heads % kv or (rows and not seqs) or (row_starts is None and seqs and rows % seqs) or max_rows < 0:
         raise IsstError(f"{what}: {rows} rows of {seqs} sequences, {heads} heads on {kv} key heads of {D} (max_rows {max_rows}) are not supported")
     a = _PrefixAttn(q.data_ptr(), k_prefix.data_ptr(), v_prefix.data_ptr(), k_tail.data_ptr(), v_tail.data_ptr(), tail_lens.data_ptr(),
@@ -820,22 +825,22 @@ def op_gemm_lora(x: torch.Tensor, packed: torch.Tensor, N: int, down: torch.Tens
     """bf16(x W^T + scales[a] (x down[a]^T) up[a]^T) with a = row_adapter[m] per row (int32; outside 0 .. n - 1: no adapter).  x (M, K) bf16, packed = op_pack_weight(W (N, K)),
     down (n, rank, K), up (n, N, rank) bf16, scales (n,) fp32; rank a multiple of 8 up to 128 (pad smaller ones with zeros), K a multiple of 32."""
     what = "op_gemm_lora"
-    lib = load_library()
-    dev = _on_device(what, x, packed=packed, down=down, up=up, scales=scales, row_adapter=row_adapter, out=out)
+    lib = _lib or load_library()
+    dev = _device_of(what, x)
     if x.dim() != 2 or down.dim() != 3:
         raise IsstError(f"{what}: x (M, K), down (n, rank, K), got {tuple(x.shape)}, {tuple(down.shape)}")
     bf = torch.bfloat16
     (M, K), (n, rank, _) = x.shape, down.shape
-    _expect(what, "x", x, bf)
-    _expect(what, "packed", packed, bf, (lib.isst_op_packed_elems(N, K),), True)
-    _expect(what, "down", down, bf, (n, rank, K), True)
-    _expect(what, "up", up, bf, (n, N, rank), True)
-    _expect(what, "scales", scales, torch.float32, (n,), True)
-    _expect(what, "row_adapter", row_adapter, torch.int32, (M,), True)
+    _expect(what, dev, "x", x, bf, (M, K), False)
+    _expect(what, dev, "packed", packed, bf, ((N + 15) // 16 * 16 * K,))
+    _expect(what, dev, "down", down, bf, (n, rank, K))
+    _expect(what, dev, "up", up, bf, (n, N, rank))
+    _expect(what, dev, "scales", scales, torch.float32, (n,))
+    _expect(what, dev, "row_adapter", row_adapter, torch.int32, (M,))
     if out is None:
         out = torch.empty((M, N), dtype=bf, device=dev)
     else:
-        _expect(what, "out", out, bf, (M, N))
+        _expect(what, dev, "out", out, bf, (M, N), False)
         if (N > 1 and out.stride(1) != 1) or (M > 1 and out.stride(0) < N):
             raise IsstError(f"{what}: rows of out must be contiguous and apart (strides {out.stride()})")
     (lda,) = _row_strides(what, "x", x)
@@ -854,28 +859,28 @@ def op_verify_drafts(target: torch.Tensor, drafts: torch.Tensor, n_drafts: Optio
     token behind the last accepted one -- or None: greedy.  Returns (tokens (streams, K + 1) int32: accepted drafts, next token, -1 behind them; counts (streams,) int32, -1 for a
     stream whose deciding row has no distribution or whose inputs are out of range)."""
     what = "op_verify_drafts"
-    lib = load_library()
-    dev = _on_device(what, target, drafts=drafts, n_drafts=n_drafts, draft_scores=draft_scores, uniforms=uniforms)
+    lib = _lib or load_library()
+    dev = _device_of(what, target)
     if target.dim() != 3 or target.shape[1] < 1 or target.shape[2] < 1:
         raise IsstError(f"{what}: target (streams, K + 1, vocab), got {tuple(target.shape)}")
     B, K, V = target.shape[0], target.shape[1] - 1, target.shape[2]
-    _expect(what, "target", target, torch.float32)
-    _expect(what, "drafts", drafts, torch.int32, (B, K), True)
+    _expect(what, dev, "target", target, torch.float32, (B, K + 1, V), False)
+    _expect(what, dev, "drafts", drafts, torch.int32, (B, K))
     if n_drafts is not None:
-        _expect(what, "n_drafts", n_drafts, torch.int32, (B,), True)
+        _expect(what, dev, "n_drafts", n_drafts, torch.int32, (B,))
     if draft_scores is not None:
-        _expect(what, "draft_scores", draft_scores, torch.float32, (B, K, V))
+        _expect(what, dev, "draft_scores", draft_scores, torch.float32, (B, K, V), False)
     if uniforms is not None:
-        _expect(what, "uniforms", uniforms, torch.float64, (B, K + 1), True)
+        _expect(what, dev, "uniforms", uniforms, torch.float64, (B, K + 1))
     if uniforms is None and draft_scores is not None:
         raise IsstError(f"{what}: greedy verification reads no draft scores")
-    for name, t in (("target", target), ("draft_scores", draft_scores)):
-        if t is not None and V > 1 and t.stride(2) != 1:
-            raise IsstError(f"{what}: rows of {name} must be contiguous (strides {t.stride()})")
+    t_st, d_st = target.stride(), (0, 0, 1) if draft_scores is None else draft_scores.stride()
+    if V > 1 and (t_st[2] != 1 or d_st[2] != 1):
+        raise IsstError(f"{what}: rows of the scores must be contiguous (strides {t_st}, {d_st})")
     tokens = torch.empty((B, K + 1), dtype=torch.int32, device=dev)
     counts = torch.empty((B,), dtype=torch.int32, device=dev)
-    ds = (None, 0, 0) if draft_scores is None else (draft_scores.data_ptr(), draft_scores.stride(0), draft_scores.stride(1))
+    ptr = lambda t: None if t is None else t.data_ptr()
     _launch(what, dev, lib.isst_op_verify_drafts_workspace(B, K, V),
-            lambda ws, n, st: lib.isst_op_verify_drafts(target.data_ptr(), target.stride(0), target.stride(1), *ds, drafts.data_ptr(), _ptr(n_drafts), _ptr(uniforms), B, K, V,
-                                                        tokens.data_ptr(), counts.data_ptr(), ws, n, st))
+            lambda ws, n, st: lib.isst_op_verify_drafts(target.data_ptr(), t_st[0], t_st[1], ptr(draft_scores), d_st[0], d_st[1], drafts.data_ptr(), ptr(n_drafts), ptr(uniforms),
+                                                        B, K, V, tokens.data_ptr(), counts.data_ptr(), ws, n, st))
     return tokens, counts

@@ -97,13 +97,17 @@ def test_python_functions_refuse_cpu_tensors_and_wrong_kinds(lib):
         E.op_gemm_lora(torch.zeros(2, 32, dtype=bf), torch.zeros(512, dtype=bf), 16, torch.zeros(1, 8, 32, dtype=bf), torch.zeros(1, 16, 8, dtype=bf), torch.zeros(1), ln)
     with pytest.raises(E.IsstError, match="GPU"):
         E.op_verify_drafts(torch.zeros(2, 3, 5), torch.zeros(2, 2, dtype=i32))
-    m = lambda *s, dt=bf: torch.empty(*s, dtype=dt, device="meta")
     # (checks behind the device's: on shapes and kinds alone)
     with pytest.raises(E.IsstError, match="must be torch.bfloat16"):
-        E._expect("op", "q", q.float(), bf)
+        E._expect("op", -1, "q", q.float(), bf, (2, 4, 128))
+    with pytest.raises(E.IsstError, match="must be torch.bfloat16"):
+        E._expect("op", -1, "q", q, bf, (2, 4, 64))
+    with pytest.raises(E.IsstError, match="expected cuda:0"):
+        E._expect("op", 0, "q", q, bf, (2, 4, 128))
     with pytest.raises(E.IsstError, match="contiguous"):
-        E._expect("op", "x", torch.zeros(4, 6).t(), torch.float32, (6, 4), True)
+        E._expect("op", -1, "x", torch.zeros(4, 6).t(), torch.float32, (6, 4))
     for view in (q.transpose(1, 2), torch.zeros(2, 4, 132, dtype=bf)[:, :, :128], torch.zeros(2 * 4 * 128 + 1, dtype=bf)[1:].view(2, 4, 128)):
         with pytest.raises(E.IsstError, match="16-byte aligned"):
             E._row_strides("op", "q", view)
-    assert E._row_strides("op", "q", q[:1]) == [0, 128] and E._row_strides("op", "k", k[:, :0]) == [0, 0]
+    odd = torch.zeros(1, 2, 129, dtype=bf)[:, :1, :128]  # strides of dims without a second entry do not count
+    assert E._row_strides("op", "q", q) == (512, 128) and E._row_strides("op", "q", odd) == (0, 0) and E._row_strides("op", "k", odd[:, :0]) == (0, 0)
