@@ -294,7 +294,13 @@ static GemmArgs lora_base_args(const uint16_t* A, int64_t lda, const uint16_t* p
     g.A = A; g.lda = lda; g.Wp = packed; g.out = base; g.N = round_up(N, 16); g.ldo = g.N; g.out_batch = (long)M * g.N;
     g.M = M; g.K = K; g.batch = 1; g.n_valid = N;
     g.epi = EPI_PARTIAL;
-    g.ksplit = M > 12 ? pick_ksplit(K, g.N, M, 1L << 28) : 1;
+    // as many K slices as give every compute unit a workgroup of that kernel, in one round
+    g.ksplit = 1;
+    if (M > 64 && !gemm_dense_would_run(M, g.N, K)) g.ksplit = pick_ksplit(K, g.N, M, 1L << 28);
+    else if (M > 12) {
+        const int blocks = M > 64 ? (g.N + 255) / 256 * ((M + 255) / 256) : (g.N + 63) / 64, step = M > 64 ? 64 : 256, least = M > 64 ? 16 : 1;
+        for (int s = 2; s <= (M > 64 ? 8 : 4) && blocks * s <= 256 && K % (step * s) == 0 && K / (step * s) >= least; s *= 2) g.ksplit = s;
+    }
     if (gemm_mid_supported(g) || gemm_tiled_supported(g)) return g;
     g.ksplit = 1;
     if (gemm_mid_supported(g) || gemm_tiled_supported(g)) return g;
@@ -302,7 +308,7 @@ static GemmArgs lora_base_args(const uint16_t* A, int64_t lda, const uint16_t* p
     return g;
 }
 static bool lora_ok(int M, int N, int K, int rank, int n_adapters) {
-    return M >= 0 && N >= 1 && N <= (1 << 24) && K >= 32 && K % 32 == 0 && K <= (1 << 24) && rank >= 8 && rank <= 128 && rank % 8 == 0 && n_adapters >= 1 &&
+    return M >= 0 && N >= 1 && N <= (1 << 21) && K >= 32 && K % 32 == 0 && K <= (1 << 24) && rank >= 8 && rank <= 128 && rank % 8 == 0 && n_adapters >= 1 &&
            (int64_t)M * N < (1L << 30) && (int64_t)M * K < (1L << 29);
 }
 extern "C" int64_t isst_op_gemm_lora_workspace(int M, int N, int K, int rank, int n_adapters) {
