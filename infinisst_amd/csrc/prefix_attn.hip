@@ -45,13 +45,13 @@ __device__ __forceinline__ int seq_of_row(const isst_prefix_attn& a, int row) {
 
 struct PrefixPlan {
     unsigned magic;                              // ceil(2^32 / G), 0 for G = 1 (group_of)
-    int prefix_block, prefix_tiles, prefix_splits, prefix_units;  // block form or span form; column tiles, key spans; units padded to a multiple of 8
+    int prefix_wide, prefix_block, prefix_tiles, prefix_splits, prefix_units;  // block form or span form; column tiles, key spans; units padded to a multiple of 8
     int own_block, own_tiles, own_splits, own_units;                           // column tiles of a sequence (a longer one walks on), key spans
     int slots;
     float* o;                                    // [slots][rows * heads][D] fp32, unnormalised
     float2* ml;                                  // [slots][rows * heads]: maximum (in units of log2), sum
 };
-// x / G for a column counted from the start of a row (x < G + 128, G < 2^15: exact)
+// x / G for a column counted from the start of a row (x < G + 256, G < 2^15: exact)
 __device__ __forceinline__ int group_of(int x, unsigned magic) { return magic ? (int)__umulhi((unsigned)x, magic) : x; }
 // what a workgroup attends to: columns c0 .. ncols - 1 of a sequence (column c = its row c / G, head kvh G + c % G) over `keys` keys; column c sees keys j < limit0 + c / G where causal
 struct KeySpan {
@@ -271,6 +271,210 @@ __device__ __forceinline__ void block_role(const isst_prefix_attn& a, const Pref
                     const int j = (see_least / PA_TILE + k) * PA_TILE;
                     add_keys<D>(a, p, w, slot, cw + c, j, j + PA_TILE);
                 }
+    }
+}
+
+// ---------------------------------------------------------------------------------------------------------------- many columns
+// The prefix for batches of many columns: 4 waves of 64 columns each, one wave per SIMD (512 registers a lane).  Against the block role a K or V fragment read from LDS feeds two matrix
+// products instead of one, and a wave has enough independent work of its own: the score product of one half tile is in flight while the vector ALU takes the exponentials of the other, the
+// value products of the first half while it takes those of the second.
+#define PW_TILE 64
+template <int D>
+__global__ __launch_bounds__(256, 1) void prefix_attn_wide_kernel(isst_prefix_attn a, PrefixPlan p) {
+    constexpr int ROWB = 2 * D, CH = D / 8, LOADS = PW_TILE * CH / 256, RSTEP = 256 / CH, QS = D / 16, DT = D / 32, STAGE = 2 * PW_TILE * ROWB;
+    __shared__ __attribute__((aligned(16))) char lds[3 * STAGE];
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), c32 = lane & 31, half = lane >> 5;
+    const int ct = (blockIdx.x >> 3) % p.prefix_tiles, g = (blockIdx.x >> 3) / p.prefix_tiles * 8 + (blockIdx.x & 7), G = a.heads / a.kv_heads;
+    const int kvh = g % a.kv_heads, split = g / a.kv_heads, ncols = a.rows * G;
+    if (split >= p.prefix_splits) return;  // (padding)
+    const int total = (a.prefix_len + PW_TILE - 1) / PW_TILE, per = (total + p.prefix_splits - 1) / p.prefix_splits, tile0 = split * per, tiles = min(per, total - tile0);
+    const int cw = ct * 256 + 64 * wave, t0 = cw / G, x0 = cw % G;
+    const bf16_t *kb = a.k_prefix + kvh * a.kp_head, *vb = a.v_prefix + kvh * a.vp_head;
+
+    const int lr = tid / CH, lc = tid % CH, kstep = (int)a.kp_key * 2, vstep = (int)a.vp_key * 2;
+    const unsigned koff = lr * kstep + lc * 16, voff = lr * vstep + lc * 16;
+    u32x4_t ks[LOADS], vs[LOADS];
+    auto fetch = [&](int i0) {
+        const int j0 = (tile0 + i0) * PW_TILE, rows = a.prefix_len - j0;
+        const __amdgpu_buffer_rsrc_t kr = key_rsrc(kb + j0 * a.kp_key), vr = key_rsrc(vb + j0 * a.vp_key);
+#pragma unroll
+        for (int i = 0; i < LOADS; ++i) {
+            ks[i] = __builtin_amdgcn_raw_buffer_load_b128(kr, lr < rows - i * RSTEP ? koff : PA_OOB, i * RSTEP * kstep, 0);
+            vs[i] = __builtin_amdgcn_raw_buffer_load_b128(vr, lr < rows - i * RSTEP ? voff : PA_OOB, i * RSTEP * vstep, 0);
+        }
+    };
+    auto put = [&](char* base) {
+#pragma unroll
+        for (int i = 0; i < LOADS; ++i) {
+            *reinterpret_cast<u32x4_t*>(base + tile_off<D>(lr + i * RSTEP, lc)) = ks[i];
+            *reinterpret_cast<u32x4_t*>(base + PW_TILE * ROWB + tile_off<D>(lr + i * RSTEP, lc)) = vs[i];
+        }
+    };
+    if (tiles > 0) fetch(0);
+    u32x4_t qf[2][QS];
+#pragma unroll
+    for (int n = 0; n < 2; ++n) {
+        const bool live = cw + 32 * n + c32 < ncols;
+        const int x = x0 + 32 * n + c32, t = live ? group_of(x, p.magic) : 0;
+#pragma unroll
+        for (int s = 0; s < QS; ++s)
+            qf[n][s] = live ? *reinterpret_cast<const u32x4_t*>(a.q + (t0 + t) * a.q_row + (kvh * G + x - t * G) * a.q_head + 16 * s + 8 * half) : (u32x4_t){0u, 0u, 0u, 0u};
+    }
+    f32x16_t o[2][DT];
+    float m[2], l[2];
+#pragma unroll
+    for (int n = 0; n < 2; ++n) {
+        m[n] = -INFINITY; l[n] = 0.f;
+#pragma unroll
+        for (int d = 0; d < DT; ++d)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) o[n][d][r] = 0.f;
+    }
+    const float c2 = a.scale * 1.44269504088896340736f;
+    if (tiles > 0) put(lds);
+    if (tiles > 1) { fetch(1); put(lds + STAGE); }
+    if (tiles > 2) fetch(2);
+    __syncthreads();
+#pragma unroll
+    for (int n = 0; n < 2; ++n)
+#pragma unroll
+        for (int s = 0; s < QS; ++s) asm volatile("" : "+v"(qf[n][s]));  // (the queries have landed)
+
+    auto scores = [&](const char* kt, f32x16_t (&sc)[2]) {  // keys of one half tile
+#pragma unroll
+        for (int n = 0; n < 2; ++n)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) sc[n][r] = 0.f;
+#pragma unroll
+        for (int s = 0; s < QS; ++s) {
+            const u32x4_t kf = *reinterpret_cast<const u32x4_t*>(kt + tile_off<D>(c32, 2 * s + half));
+#pragma unroll
+            for (int n = 0; n < 2; ++n) sc[n] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8_t, kf), __builtin_bit_cast(bf16x8_t, qf[n][s]), sc[n], 0, 0, 0);
+        }
+    };
+    auto values = [&](const char* vt, const u32x4_t (&pf)[2][2]) {
+#pragma unroll
+        for (int k = 0; k < 2; ++k)  // 16 keys: slots j < 4 of half h = keys 16 k + 4 h + j, j >= 4 = keys 16 k + 8 + 4 h + (j - 4)
+#pragma unroll
+            for (int d = 0; d < DT; ++d) {
+                const int ch = 4 * d + 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1), r = 16 * k + 4 * half + ((lane >> 2) & 3);
+                const u32x2_t v1 = read_tr(vt + tile_off<D>(r, ch) + 8 * (lane & 1)), v2 = read_tr(vt + tile_off<D>(r + 8, ch) + 8 * (lane & 1));
+                const u32x4_t vf = {v1.x, v1.y, v2.x, v2.y};
+#pragma unroll
+                for (int n = 0; n < 2; ++n)
+                    o[n][d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8_t, vf), __builtin_bit_cast(bf16x8_t, pf[n][k]), o[n][d], 0, 0, 0);
+            }
+    };
+    auto hide = [&](int rows, f32x16_t (&sc)[2]) {  // keys behind the prefix (rows: live keys of this half tile)
+#pragma unroll
+        for (int n = 0; n < 2; ++n)
+#pragma unroll
+            for (int r = 0; r < 16; ++r)
+                if ((r & 3) + 8 * (r >> 2) + 4 * half >= rows) sc[n][r] = -INFINITY;
+    };
+    // weights of a half tile (bf16 pairs in the layout of the value product) and their sum per lane, as the product will see them
+    auto weights = [&](const f32x16_t (&sc)[2], u32x4_t (&pf)[2][2], float (&sum)[2]) {
+#pragma unroll
+        for (int n = 0; n < 2; ++n) {
+            const float neg = m[n] == -INFINITY ? 0.f : -m[n];
+            const bf16x2_t one = {(__bf16)1.f, (__bf16)1.f};
+            sum[n] = 0.f;
+#pragma unroll
+            for (int k = 0; k < 2; ++k)
+#pragma unroll
+                for (int w = 0; w < 4; ++w) {
+                    const int r = 8 * k + 2 * w;
+                    const uint32_t pair = pack_bf(__builtin_amdgcn_exp2f(__builtin_fmaf(sc[n][r], c2, neg)), __builtin_amdgcn_exp2f(__builtin_fmaf(sc[n][r + 1], c2, neg)));
+                    pf[n][k][w] = pair;
+                    sum[n] = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2_t, pair), one, sum[n], false);
+                }
+        }
+    };
+    // m becomes the maximum of what it covers and of these scores
+    auto raise = [&](const f32x16_t (&sc)[2]) {
+#pragma unroll
+        for (int n = 0; n < 2; ++n) {
+            float mx = sc[n][0];
+#pragma unroll
+            for (int r = 1; r < 16; ++r) mx = fmaxf(mx, sc[n][r]);
+            mx = fmaxf(mx, __shfl_xor(mx, 32, WAVE)) * c2;
+            const float m2 = fmaxf(m[n], mx), keep = m[n] == m2 ? 1.f : m[n] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m[n] - m2);
+            l[n] *= keep;
+#pragma unroll
+            for (int d = 0; d < DT; ++d)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) o[n][d][r] *= keep;
+            m[n] = m2;
+        }
+    };
+    // A column's reference m is the maximum of its first half tile: weights are exponentials against it, bf16 and fp32 hold them to 2^127, and no bit is lost by their size.  So later
+    // maxima are not looked for; only a half tile whose weights pass 2^60 (or hold NaN) moves m, before anything of it was used.
+    auto settle = [&](const f32x16_t (&sc)[2], u32x4_t (&pf)[2][2], float (&sum)[2]) {
+        if (__any(!(sum[0] <= 0x1p60f) || !(sum[1] <= 0x1p60f))) {
+            raise(sc);
+            weights(sc, pf, sum);
+        }
+        l[0] += sum[0];
+        l[1] += sum[1];
+    };
+    f32x16_t sa[2], sb[2];
+    scores(lds, sa);
+    if (a.prefix_len - tile0 * PW_TILE < 32) hide(a.prefix_len - tile0 * PW_TILE, sa);
+    raise(sa);
+    char *cur = lds, *next = lds + STAGE, *spare = lds + 2 * STAGE;
+    auto step = [&](int i, auto last) {
+        constexpr bool LAST = decltype(last)::value;
+        const char* vt = cur + PW_TILE * ROWB;
+        const int rows = a.prefix_len - (tile0 + i) * PW_TILE;
+        u32x4_t pa[2][2], pb[2][2];
+        float ta[2], tb[2];
+        if constexpr (LAST) hide(rows, sa);
+        scores(cur + 32 * ROWB, sb);
+        weights(sa, pa, ta);
+        settle(sa, pa, ta);
+        if (i + 2 < tiles) put(spare);
+        if constexpr (LAST) hide(rows - 32, sb);
+        values(vt, pa);
+        weights(sb, pb, tb);
+        settle(sb, pb, tb);
+        if (i + 3 < tiles) fetch(i + 3);
+        values(vt + 32 * ROWB, pb);
+        scores(next, sa);  // (behind the last tile: of whatever the stage holds, unused)
+        __syncthreads();
+        char* done = cur;
+        cur = next; next = spare; spare = done;
+    };
+    const int whole = (tile0 + tiles) * PW_TILE <= a.prefix_len ? tiles : tiles - 1;
+    int i = 0;
+    for (; i < whole; ++i) step(i, std::integral_constant<bool, false>{});
+    for (; i < tiles; ++i) step(i, std::integral_constant<bool, true>{});
+
+    const long base = (long)split * a.rows * a.heads;
+    float* red = reinterpret_cast<float*>(lds) + wave * (32 * D);
+#pragma unroll
+    for (int n = 0; n < 2; ++n) {
+        const int c0 = cw + 32 * n;
+        l[n] += __shfl_xor(l[n], 32, WAVE);
+        if (half == 0 && c0 + c32 < ncols) {
+            const int x = x0 + 32 * n + c32, t = group_of(x, p.magic);
+            p.ml[base + (long)(t0 + t) * a.heads + kvh * G + x - t * G] = make_float2(m[n], l[n]);
+        }
+        __builtin_amdgcn_wave_barrier();
+#pragma unroll
+        for (int d = 0; d < DT; ++d)
+#pragma unroll
+            for (int r4 = 0; r4 < 4; ++r4) {
+                const int d4 = 8 * d + 2 * r4 + half;
+                *reinterpret_cast<f32x4_t*>(red + c32 * D + 4 * (d4 ^ (c32 & (D / 4 - 1)))) = (f32x4_t){o[n][d][4 * r4], o[n][d][4 * r4 + 1], o[n][d][4 * r4 + 2], o[n][d][4 * r4 + 3]};
+            }
+        __builtin_amdgcn_wave_barrier();
+        constexpr int L4 = D / 4, CPI = 64 / L4;
+        const int d4 = lane % L4;
+        for (int c = lane / L4; c < 32; c += CPI) {
+            if (c0 + c >= ncols) break;
+            const int x = x0 + 32 * n + c, t = group_of(x, p.magic);
+            *reinterpret_cast<f32x4_t*>(p.o + (base + (long)(t0 + t) * a.heads + kvh * G + x - t * G) * D + 4 * d4) = *reinterpret_cast<const f32x4_t*>(red + c * D + 4 * (d4 ^ (c & (L4 - 1))));
+        }
     }
 }
 
@@ -540,6 +744,12 @@ __global__ __launch_bounds__(256) void prefix_attn_join_kernel(isst_prefix_attn 
 #ifndef PA_TAU
 #define PA_TAU 1.25
 #endif
+#ifndef PA_WIDE
+#define PA_WIDE 512
+#endif
+#ifndef PW_TAU
+#define PW_TAU 1.8
+#endif
 #ifndef PA_FIX
 #define PA_FIX 5.0
 #endif
@@ -572,17 +782,19 @@ static PrefixPlan plan(const isst_prefix_attn& a) {
     }
     if (a.prefix_len > 0) {
         p.prefix_block = cols > 32;
-        p.prefix_tiles = p.prefix_block ? ceil_div(cols, width) : 1;
+        p.prefix_wide = cols >= PA_WIDE;
+        p.prefix_tiles = p.prefix_wide ? ceil_div(cols, 256) : p.prefix_block ? ceil_div(cols, width) : 1;
         if (p.prefix_block) {
             // key spans: the rounds of the chip that the units take (with the own keys' units filling what a last round leaves) + what their partial results cost
-            const int tiles = ceil_div(a.prefix_len, PA_TILE), groups = a.kv_heads * p.prefix_tiles;
+            const double tau = p.prefix_wide ? PW_TAU : PA_TAU, slots_now = p.prefix_wide ? 256 : room;
+            const int tiles = ceil_div(a.prefix_len, p.prefix_wide ? PW_TILE : PA_TILE), groups = a.kv_heads * p.prefix_tiles;
             double best = 1e30;
             for (int s = 1; s <= PA_MAX_SLOTS - 8 && s <= tiles; ++s) {
                 const int per = ceil_div(tiles, s);
                 if (ceil_div(tiles, per) != s) continue;
-                const double dur = per * PA_TAU * (a.head_dim / 128.0) + PA_FIX, units = (double)groups * s;
-                const double even = (units * dur + own_us) / room, rounds = dur * ceil_div((long)units, (long)room);
-                const double t = (even > rounds ? even : rounds) + s * (double)a.rows * a.heads * (8.0 * a.head_dim) / 3e6;
+                const double dur = per * tau * (a.head_dim / 128.0) + PA_FIX, units = (double)groups * s;
+                const double even = (units * dur + own_us) / slots_now, rounds = dur * ceil_div((long)units, (long)slots_now);
+                const double t = (even > rounds && !p.prefix_wide ? even : rounds) + s * (double)a.rows * a.heads * (8.0 * a.head_dim) / 3e6;
                 if (t < best) { best = t; p.prefix_splits = s; }
             }
         } else {
@@ -607,6 +819,11 @@ int launch_prefix_attention(const isst_prefix_attn& a, void* workspace, hipStrea
     p.o = static_cast<float*>(workspace);
     p.ml = reinterpret_cast<float2*>(p.o + p.slots * pairs * a.head_dim);
     const int nq = span_nq(a);
+    if (p.prefix_wide) {
+        if (a.head_dim == 128) hipLaunchKernelGGL(prefix_attn_wide_kernel<128>, dim3((unsigned)p.prefix_units), dim3(256), 0, s, a, p);
+        else hipLaunchKernelGGL(prefix_attn_wide_kernel<64>, dim3((unsigned)p.prefix_units), dim3(256), 0, s, a, p);
+        p.prefix_units = 0;
+    }
     if (p.prefix_units + p.own_units > 0) {
         if (a.head_dim == 128) { if (nq == 1) launch_partial<128, 1>(a, p, s); else launch_partial<128, 2>(a, p, s); }
         else { if (nq == 1) launch_partial<64, 1>(a, p, s); else launch_partial<64, 2>(a, p, s); }
