@@ -45,13 +45,13 @@ __device__ __forceinline__ int seq_of_row(const isst_prefix_attn& a, int row) {
 
 struct PrefixPlan {
     unsigned magic;                              // ceil(2^32 / G), 0 for G = 1 (group_of)
-    int prefix_wide, prefix_block, prefix_tiles, prefix_splits, prefix_units;  // block form or span form; column tiles, key spans; units padded to a multiple of 8
+    int prefix_block, prefix_tiles, prefix_splits, prefix_units;  // block form or span form; column tiles, key spans; units padded to a multiple of 8
     int own_block, own_tiles, own_splits, own_units;                           // column tiles of a sequence (a longer one walks on), key spans
     int slots;
     float* o;                                    // [slots][rows * heads][D] fp32, unnormalised
     float2* ml;                                  // [slots][rows * heads]: maximum (in units of log2), sum
 };
-// x / G for a column counted from the start of a row (x < G + 256, G < 2^15: exact)
+// x / G for a column counted from the start of a row (x < G + 128, G < 2^15: exact)
 __device__ __forceinline__ int group_of(int x, unsigned magic) { return magic ? (int)__umulhi((unsigned)x, magic) : x; }
 // what a workgroup attends to: columns c0 .. ncols - 1 of a sequence (column c = its row c / G, head kvh G + c % G) over `keys` keys; column c sees keys j < limit0 + c / G where causal
 struct KeySpan {
@@ -112,24 +112,26 @@ __device__ __forceinline__ void block_role(const isst_prefix_attn& a, const Pref
 
     const int lr = tid / CH, lc = tid % CH, kstep = (int)w.kstride * 2, vstep = (int)w.vstride * 2;
     const unsigned koff = lr * kstep + lc * 16, voff = lr * vstep + lc * 16;
-    u32x4_t ks[LOADS], vs[LOADS];
-    auto fetch = [&](int i0) {
+    struct Rows { u32x4_t k[LOADS], v[LOADS]; };
+    auto fetch = [&](Rows& x, int i0) {
         const int j0 = (tile0 + i0) * PA_TILE, rows = w.keys - j0;
         const __amdgpu_buffer_rsrc_t kr = key_rsrc(w.k + j0 * w.kstride), vr = key_rsrc(w.v + j0 * w.vstride);
 #pragma unroll
         for (int i = 0; i < LOADS; ++i) {
-            ks[i] = __builtin_amdgcn_raw_buffer_load_b128(kr, lr < rows - i * RSTEP ? koff : PA_OOB, i * RSTEP * kstep, 0);
-            vs[i] = __builtin_amdgcn_raw_buffer_load_b128(vr, lr < rows - i * RSTEP ? voff : PA_OOB, i * RSTEP * vstep, 0);
+            x.k[i] = __builtin_amdgcn_raw_buffer_load_b128(kr, lr < rows - i * RSTEP ? koff : PA_OOB, i * RSTEP * kstep, 0);
+            x.v[i] = __builtin_amdgcn_raw_buffer_load_b128(vr, lr < rows - i * RSTEP ? voff : PA_OOB, i * RSTEP * vstep, 0);
         }
     };
-    auto put = [&](char* base) {
+    auto put = [&](const Rows& x, char* base) {
 #pragma unroll
         for (int i = 0; i < LOADS; ++i) {
-            *reinterpret_cast<u32x4_t*>(base + tile_off<D>(lr + i * RSTEP, lc)) = ks[i];
-            *reinterpret_cast<u32x4_t*>(base + PA_TILE * ROWB + tile_off<D>(lr + i * RSTEP, lc)) = vs[i];
+            *reinterpret_cast<u32x4_t*>(base + tile_off<D>(lr + i * RSTEP, lc)) = x.k[i];
+            *reinterpret_cast<u32x4_t*>(base + PA_TILE * ROWB + tile_off<D>(lr + i * RSTEP, lc)) = x.v[i];
         }
     };
-    if (tiles > 0) fetch(0);
+    Rows staged, second;
+    if (tiles > 0) fetch(staged, 0);
+    if (tiles > 1) fetch(second, 1);
     u32x4_t qf[QS];
 #pragma unroll
     for (int s = 0; s < QS; ++s)
@@ -144,9 +146,9 @@ __device__ __forceinline__ void block_role(const isst_prefix_attn& a, const Pref
     const float c2 = a.scale * 1.44269504088896340736f;  // exp(scale s - ..) = exp2(c2 s - ..)
 
     char *cur = lds, *next = lds + STAGE, *spare = lds + 2 * STAGE;
-    if (tiles > 0) put(cur);
-    if (tiles > 1) { fetch(1); put(next); }
-    if (tiles > 2) fetch(2);
+    if (tiles > 0) put(staged, cur);
+    if (tiles > 2) fetch(staged, 2);
+    if (tiles > 1) put(second, next);
     __syncthreads();
 #pragma unroll
     for (int s = 0; s < QS; ++s) asm volatile("" : "+v"(qf[s]));  // (the queries have landed: a wait for them inside the loop would wait for the newest tile as well)
@@ -163,42 +165,60 @@ __device__ __forceinline__ void block_role(const isst_prefix_attn& a, const Pref
     };
     f32x16_t sc = scores(cur);  // (no tile: of whatever the stage holds, unused -- as behind the last tile below)
     auto stage = [&](int i) {
-        if (i + 2 < tiles) put(spare);
-        if (i + 3 < tiles) fetch(i + 3);
+        if (i + 2 < tiles) put(staged, spare);
+        if (i + 3 < tiles) fetch(staged, i + 3);
     };
     auto turn = [&]() {
         __syncthreads();
         char* done = cur;
         cur = next; next = spare; spare = done;
     };
-    // one tile: its scores are in sc, those of the next are computed on the way.  EDGE: some column does not see some key of it
+    // m becomes the maximum of what it covers and of these scores
+    auto raise = [&]() {
+        float mx = sc[0];
+#pragma unroll
+        for (int r = 1; r < 16; ++r) mx = fmaxf(mx, sc[r]);
+        mx = fmaxf(mx, __shfl_xor(mx, 32, WAVE)) * c2;
+        const float m2 = fmaxf(m, mx), keep = m == m2 ? 1.f : m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - m2);
+        l *= keep;
+#pragma unroll
+        for (int d = 0; d < DT; ++d)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) o[d][r] *= keep;
+        m = m2;
+    };
+    // weights of the tile (bf16 pairs in the layout of the value product) and their sum in this lane, as the product will see them
+    auto weights = [&](u32x4_t (&pf)[2]) {
+        const float neg = m == -INFINITY ? 0.f : -m;
+        const bf16x2_t one = {(__bf16)1.f, (__bf16)1.f};
+        float sum = 0.f;
+#pragma unroll
+        for (int k = 0; k < 2; ++k)
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                const int r = 8 * k + 2 * q;
+                const uint32_t pair = pack_bf(__builtin_amdgcn_exp2f(__builtin_fmaf(sc[r], c2, neg)), __builtin_amdgcn_exp2f(__builtin_fmaf(sc[r + 1], c2, neg)));
+                pf[k][q] = pair;
+                sum = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2_t, pair), one, sum, false);
+            }
+        return sum;
+    };
+    // One tile: its scores are in sc, those of the next are computed on the way.  EDGE: some column does not see some key of it.
+    // A column's reference m is the maximum of its first tile (and of its edge tiles): weights are exponentials against it, bf16 and fp32 hold them to 2^127, and no bit is lost by their
+    // size.  So other maxima are not looked for -- that and the running sum were 100 of the 169 vector instructions of a tile -- and only weights that pass 2^60 (or NaN) move m,
+    // before anything of the tile was used.
     auto step = [&](int i, auto edge) {
         constexpr bool EDGE = decltype(edge)::value;
         stage(i);
         const char* vt = cur + PA_TILE * ROWB;
         const int j0 = (tile0 + i) * PA_TILE;
+        bool ill = false;  // inf or NaN among the values
         if constexpr (EDGE) {
             const int lim = limit - j0 - 4 * half;
 #pragma unroll
             for (int r = 0; r < 16; ++r)
                 if ((r & 3) + 8 * (r >> 2) >= lim) sc[r] = -INFINITY;
-        }
-        float mx = sc[0];
-#pragma unroll
-        for (int r = 1; r < 16; ++r) mx = fmaxf(mx, sc[r]);
-        mx = fmaxf(mx, __shfl_xor(mx, 32, WAVE)) * c2;
-        if (__any(mx > m)) {
-            const float m2 = fmaxf(m, mx), keep = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - m2);
-            l *= keep;
-#pragma unroll
-            for (int d = 0; d < DT; ++d)
-#pragma unroll
-                for (int r = 0; r < 16; ++r) o[d][r] *= keep;
-            m = m2;
-        }
-        const float neg = m == -INFINITY ? 0.f : -m;
-        bool ill = false;  // inf or NaN among the values
-        if constexpr (EDGE) {
+            raise();
 #pragma unroll 1
             for (int k = 0; k < PA_TILE * ROWB / 1024; ++k) {
                 const u32x4_t v = *reinterpret_cast<const u32x4_t*>(vt + 1024 * k + 16 * lane);
@@ -207,17 +227,15 @@ __device__ __forceinline__ void block_role(const isst_prefix_attn& a, const Pref
             }
             ill = __any(ill);
         }
-        const f32x16_t sn = scores(next);
         u32x4_t pf[2];
-        float e[16];
-#pragma unroll
-        for (int r = 0; r < 16; ++r) {
-            e[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[r], c2, neg));
-            l += e[r];
-        }
-#pragma unroll
-        for (int k = 0; k < 2; ++k)
-            pf[k] = (u32x4_t){pack_bf(e[8 * k], e[8 * k + 1]), pack_bf(e[8 * k + 2], e[8 * k + 3]), pack_bf(e[8 * k + 4], e[8 * k + 5]), pack_bf(e[8 * k + 6], e[8 * k + 7])};
+        float sum = weights(pf);
+        if constexpr (!EDGE)
+            if (__any(!(sum <= 0x1p60f))) {
+                raise();
+                sum = weights(pf);
+            }
+        l += sum;
+        const f32x16_t sn = scores(next);
         if (!EDGE || !ill) {
 #pragma unroll
             for (int k = 0; k < 2; ++k)  // 16 keys: slots j < 4 of half h = keys 16 k + 4 h + j, j >= 4 = keys 16 k + 8 + 4 h + (j - 4)
@@ -235,6 +253,7 @@ __device__ __forceinline__ void block_role(const isst_prefix_attn& a, const Pref
         turn();
     };
     const int whole = min(mine, see_least / PA_TILE - tile0);  // tiles that every column of the wave sees whole
+    if (whole > 0) raise();
     int i = 0;
     for (; i < whole; ++i) step(i, std::integral_constant<bool, false>{});
     for (; i < mine; ++i) step(i, std::integral_constant<bool, true>{});
@@ -271,210 +290,6 @@ __device__ __forceinline__ void block_role(const isst_prefix_attn& a, const Pref
                     const int j = (see_least / PA_TILE + k) * PA_TILE;
                     add_keys<D>(a, p, w, slot, cw + c, j, j + PA_TILE);
                 }
-    }
-}
-
-// ---------------------------------------------------------------------------------------------------------------- many columns
-// The prefix for batches of many columns: 4 waves of 64 columns each, one wave per SIMD (512 registers a lane).  Against the block role a K or V fragment read from LDS feeds two matrix
-// products instead of one, and a wave has enough independent work of its own: the score product of one half tile is in flight while the vector ALU takes the exponentials of the other, the
-// value products of the first half while it takes those of the second.
-#define PW_TILE 64
-template <int D>
-__global__ __launch_bounds__(256, 1) void prefix_attn_wide_kernel(isst_prefix_attn a, PrefixPlan p) {
-    constexpr int ROWB = 2 * D, CH = D / 8, LOADS = PW_TILE * CH / 256, RSTEP = 256 / CH, QS = D / 16, DT = D / 32, STAGE = 2 * PW_TILE * ROWB;
-    __shared__ __attribute__((aligned(16))) char lds[3 * STAGE];
-    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), c32 = lane & 31, half = lane >> 5;
-    const int ct = (blockIdx.x >> 3) % p.prefix_tiles, g = (blockIdx.x >> 3) / p.prefix_tiles * 8 + (blockIdx.x & 7), G = a.heads / a.kv_heads;
-    const int kvh = g % a.kv_heads, split = g / a.kv_heads, ncols = a.rows * G;
-    if (split >= p.prefix_splits) return;  // (padding)
-    const int total = (a.prefix_len + PW_TILE - 1) / PW_TILE, per = (total + p.prefix_splits - 1) / p.prefix_splits, tile0 = split * per, tiles = min(per, total - tile0);
-    const int cw = ct * 256 + 64 * wave, t0 = cw / G, x0 = cw % G;
-    const bf16_t *kb = a.k_prefix + kvh * a.kp_head, *vb = a.v_prefix + kvh * a.vp_head;
-
-    const int lr = tid / CH, lc = tid % CH, kstep = (int)a.kp_key * 2, vstep = (int)a.vp_key * 2;
-    const unsigned koff = lr * kstep + lc * 16, voff = lr * vstep + lc * 16;
-    u32x4_t ks[LOADS], vs[LOADS];
-    auto fetch = [&](int i0) {
-        const int j0 = (tile0 + i0) * PW_TILE, rows = a.prefix_len - j0;
-        const __amdgpu_buffer_rsrc_t kr = key_rsrc(kb + j0 * a.kp_key), vr = key_rsrc(vb + j0 * a.vp_key);
-#pragma unroll
-        for (int i = 0; i < LOADS; ++i) {
-            ks[i] = __builtin_amdgcn_raw_buffer_load_b128(kr, lr < rows - i * RSTEP ? koff : PA_OOB, i * RSTEP * kstep, 0);
-            vs[i] = __builtin_amdgcn_raw_buffer_load_b128(vr, lr < rows - i * RSTEP ? voff : PA_OOB, i * RSTEP * vstep, 0);
-        }
-    };
-    auto put = [&](char* base) {
-#pragma unroll
-        for (int i = 0; i < LOADS; ++i) {
-            *reinterpret_cast<u32x4_t*>(base + tile_off<D>(lr + i * RSTEP, lc)) = ks[i];
-            *reinterpret_cast<u32x4_t*>(base + PW_TILE * ROWB + tile_off<D>(lr + i * RSTEP, lc)) = vs[i];
-        }
-    };
-    if (tiles > 0) fetch(0);
-    u32x4_t qf[2][QS];
-#pragma unroll
-    for (int n = 0; n < 2; ++n) {
-        const bool live = cw + 32 * n + c32 < ncols;
-        const int x = x0 + 32 * n + c32, t = live ? group_of(x, p.magic) : 0;
-#pragma unroll
-        for (int s = 0; s < QS; ++s)
-            qf[n][s] = live ? *reinterpret_cast<const u32x4_t*>(a.q + (t0 + t) * a.q_row + (kvh * G + x - t * G) * a.q_head + 16 * s + 8 * half) : (u32x4_t){0u, 0u, 0u, 0u};
-    }
-    f32x16_t o[2][DT];
-    float m[2], l[2];
-#pragma unroll
-    for (int n = 0; n < 2; ++n) {
-        m[n] = -INFINITY; l[n] = 0.f;
-#pragma unroll
-        for (int d = 0; d < DT; ++d)
-#pragma unroll
-            for (int r = 0; r < 16; ++r) o[n][d][r] = 0.f;
-    }
-    const float c2 = a.scale * 1.44269504088896340736f;
-    if (tiles > 0) put(lds);
-    if (tiles > 1) { fetch(1); put(lds + STAGE); }
-    if (tiles > 2) fetch(2);
-    __syncthreads();
-#pragma unroll
-    for (int n = 0; n < 2; ++n)
-#pragma unroll
-        for (int s = 0; s < QS; ++s) asm volatile("" : "+v"(qf[n][s]));  // (the queries have landed)
-
-    auto scores = [&](const char* kt, f32x16_t (&sc)[2]) {  // keys of one half tile
-#pragma unroll
-        for (int n = 0; n < 2; ++n)
-#pragma unroll
-            for (int r = 0; r < 16; ++r) sc[n][r] = 0.f;
-#pragma unroll
-        for (int s = 0; s < QS; ++s) {
-            const u32x4_t kf = *reinterpret_cast<const u32x4_t*>(kt + tile_off<D>(c32, 2 * s + half));
-#pragma unroll
-            for (int n = 0; n < 2; ++n) sc[n] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8_t, kf), __builtin_bit_cast(bf16x8_t, qf[n][s]), sc[n], 0, 0, 0);
-        }
-    };
-    auto values = [&](const char* vt, const u32x4_t (&pf)[2][2]) {
-#pragma unroll
-        for (int k = 0; k < 2; ++k)  // 16 keys: slots j < 4 of half h = keys 16 k + 4 h + j, j >= 4 = keys 16 k + 8 + 4 h + (j - 4)
-#pragma unroll
-            for (int d = 0; d < DT; ++d) {
-                const int ch = 4 * d + 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1), r = 16 * k + 4 * half + ((lane >> 2) & 3);
-                const u32x2_t v1 = read_tr(vt + tile_off<D>(r, ch) + 8 * (lane & 1)), v2 = read_tr(vt + tile_off<D>(r + 8, ch) + 8 * (lane & 1));
-                const u32x4_t vf = {v1.x, v1.y, v2.x, v2.y};
-#pragma unroll
-                for (int n = 0; n < 2; ++n)
-                    o[n][d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8_t, vf), __builtin_bit_cast(bf16x8_t, pf[n][k]), o[n][d], 0, 0, 0);
-            }
-    };
-    auto hide = [&](int rows, f32x16_t (&sc)[2]) {  // keys behind the prefix (rows: live keys of this half tile)
-#pragma unroll
-        for (int n = 0; n < 2; ++n)
-#pragma unroll
-            for (int r = 0; r < 16; ++r)
-                if ((r & 3) + 8 * (r >> 2) + 4 * half >= rows) sc[n][r] = -INFINITY;
-    };
-    // weights of a half tile (bf16 pairs in the layout of the value product) and their sum per lane, as the product will see them
-    auto weights = [&](const f32x16_t (&sc)[2], u32x4_t (&pf)[2][2], float (&sum)[2]) {
-#pragma unroll
-        for (int n = 0; n < 2; ++n) {
-            const float neg = m[n] == -INFINITY ? 0.f : -m[n];
-            const bf16x2_t one = {(__bf16)1.f, (__bf16)1.f};
-            sum[n] = 0.f;
-#pragma unroll
-            for (int k = 0; k < 2; ++k)
-#pragma unroll
-                for (int w = 0; w < 4; ++w) {
-                    const int r = 8 * k + 2 * w;
-                    const uint32_t pair = pack_bf(__builtin_amdgcn_exp2f(__builtin_fmaf(sc[n][r], c2, neg)), __builtin_amdgcn_exp2f(__builtin_fmaf(sc[n][r + 1], c2, neg)));
-                    pf[n][k][w] = pair;
-                    sum[n] = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2_t, pair), one, sum[n], false);
-                }
-        }
-    };
-    // m becomes the maximum of what it covers and of these scores
-    auto raise = [&](const f32x16_t (&sc)[2]) {
-#pragma unroll
-        for (int n = 0; n < 2; ++n) {
-            float mx = sc[n][0];
-#pragma unroll
-            for (int r = 1; r < 16; ++r) mx = fmaxf(mx, sc[n][r]);
-            mx = fmaxf(mx, __shfl_xor(mx, 32, WAVE)) * c2;
-            const float m2 = fmaxf(m[n], mx), keep = m[n] == m2 ? 1.f : m[n] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m[n] - m2);
-            l[n] *= keep;
-#pragma unroll
-            for (int d = 0; d < DT; ++d)
-#pragma unroll
-                for (int r = 0; r < 16; ++r) o[n][d][r] *= keep;
-            m[n] = m2;
-        }
-    };
-    // A column's reference m is the maximum of its first half tile: weights are exponentials against it, bf16 and fp32 hold them to 2^127, and no bit is lost by their size.  So later
-    // maxima are not looked for; only a half tile whose weights pass 2^60 (or hold NaN) moves m, before anything of it was used.
-    auto settle = [&](const f32x16_t (&sc)[2], u32x4_t (&pf)[2][2], float (&sum)[2]) {
-        if (__any(!(sum[0] <= 0x1p60f) || !(sum[1] <= 0x1p60f))) {
-            raise(sc);
-            weights(sc, pf, sum);
-        }
-        l[0] += sum[0];
-        l[1] += sum[1];
-    };
-    f32x16_t sa[2], sb[2];
-    scores(lds, sa);
-    if (a.prefix_len - tile0 * PW_TILE < 32) hide(a.prefix_len - tile0 * PW_TILE, sa);
-    raise(sa);
-    char *cur = lds, *next = lds + STAGE, *spare = lds + 2 * STAGE;
-    auto step = [&](int i, auto last) {
-        constexpr bool LAST = decltype(last)::value;
-        const char* vt = cur + PW_TILE * ROWB;
-        const int rows = a.prefix_len - (tile0 + i) * PW_TILE;
-        u32x4_t pa[2][2], pb[2][2];
-        float ta[2], tb[2];
-        if constexpr (LAST) hide(rows, sa);
-        scores(cur + 32 * ROWB, sb);
-        weights(sa, pa, ta);
-        settle(sa, pa, ta);
-        if (i + 2 < tiles) put(spare);
-        if constexpr (LAST) hide(rows - 32, sb);
-        values(vt, pa);
-        weights(sb, pb, tb);
-        settle(sb, pb, tb);
-        if (i + 3 < tiles) fetch(i + 3);
-        values(vt + 32 * ROWB, pb);
-        scores(next, sa);  // (behind the last tile: of whatever the stage holds, unused)
-        __syncthreads();
-        char* done = cur;
-        cur = next; next = spare; spare = done;
-    };
-    const int whole = (tile0 + tiles) * PW_TILE <= a.prefix_len ? tiles : tiles - 1;
-    int i = 0;
-    for (; i < whole; ++i) step(i, std::integral_constant<bool, false>{});
-    for (; i < tiles; ++i) step(i, std::integral_constant<bool, true>{});
-
-    const long base = (long)split * a.rows * a.heads;
-    float* red = reinterpret_cast<float*>(lds) + wave * (32 * D);
-#pragma unroll
-    for (int n = 0; n < 2; ++n) {
-        const int c0 = cw + 32 * n;
-        l[n] += __shfl_xor(l[n], 32, WAVE);
-        if (half == 0 && c0 + c32 < ncols) {
-            const int x = x0 + 32 * n + c32, t = group_of(x, p.magic);
-            p.ml[base + (long)(t0 + t) * a.heads + kvh * G + x - t * G] = make_float2(m[n], l[n]);
-        }
-        __builtin_amdgcn_wave_barrier();
-#pragma unroll
-        for (int d = 0; d < DT; ++d)
-#pragma unroll
-            for (int r4 = 0; r4 < 4; ++r4) {
-                const int d4 = 8 * d + 2 * r4 + half;
-                *reinterpret_cast<f32x4_t*>(red + c32 * D + 4 * (d4 ^ (c32 & (D / 4 - 1)))) = (f32x4_t){o[n][d][4 * r4], o[n][d][4 * r4 + 1], o[n][d][4 * r4 + 2], o[n][d][4 * r4 + 3]};
-            }
-        __builtin_amdgcn_wave_barrier();
-        constexpr int L4 = D / 4, CPI = 64 / L4;
-        const int d4 = lane % L4;
-        for (int c = lane / L4; c < 32; c += CPI) {
-            if (c0 + c >= ncols) break;
-            const int x = x0 + 32 * n + c, t = group_of(x, p.magic);
-            *reinterpret_cast<f32x4_t*>(p.o + (base + (long)(t0 + t) * a.heads + kvh * G + x - t * G) * D + 4 * d4) = *reinterpret_cast<const f32x4_t*>(red + c * D + 4 * (d4 ^ (c & (L4 - 1))));
-        }
     }
 }
 
@@ -530,6 +345,7 @@ __device__ __forceinline__ void span_role(const isst_prefix_attn& a, const Prefi
         for (int t = 0; t < NT; ++t) o[n][t] = (f32x4_t){0.f, 0.f, 0.f, 0.f};
     }
     const float c2 = a.scale * 1.44269504088896340736f;
+    bool first_step = true;
     for (; j0 < see_most; j0 += step) {
 #pragma unroll
         for (int i = 0; i < VL; ++i) *reinterpret_cast<u32x4_t*>(vl + tile_off<D>(i * VR + lane / CH, lane % CH)) = vr[i];
@@ -550,40 +366,62 @@ __device__ __forceinline__ void span_role(const isst_prefix_attn& a, const Prefi
         if (more) fetch_k(j0 + step);
         __builtin_amdgcn_sched_barrier(0);
         const bool edge = j0 + 32 > see_least;  // some column does not see some key of this step
-        u32x4_t pf[NQ];
+        auto raise = [&]() {  // m becomes the maximum of what it covers and of these scores
 #pragma unroll
-        for (int n = 0; n < NQ; ++n) {
-            if (edge) {
+            for (int n = 0; n < NQ; ++n) {
+                float mx = sc[n][0][0];
+#pragma unroll
+                for (int t = 0; t < 2; ++t)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) mx = fmaxf(mx, sc[n][t][r]);
+                mx = fmaxf(mx, __shfl_xor(mx, 16, WAVE));
+                mx = fmaxf(mx, __shfl_xor(mx, 32, WAVE)) * c2;
+                const float m2 = fmaxf(m[n], mx), keep = m[n] == m2 ? 1.f : m[n] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m[n] - m2);
+                l[n] *= keep;
+#pragma unroll
+                for (int t = 0; t < NT; ++t)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) o[n][t][r] *= keep;
+                m[n] = m2;
+            }
+        };
+        if (edge) {
+#pragma unroll
+            for (int n = 0; n < NQ; ++n)
 #pragma unroll
                 for (int t = 0; t < 2; ++t)
 #pragma unroll
                     for (int r = 0; r < 4; ++r)
                         if (j0 + 16 * t + 4 * fq + r >= limit[n]) sc[n][t][r] = -INFINITY;
-            }
-            float mx = -INFINITY;
-#pragma unroll
-            for (int t = 0; t < 2; ++t)
-#pragma unroll
-                for (int r = 0; r < 4; ++r) mx = fmaxf(mx, sc[n][t][r]);
-            mx = fmaxf(mx, __shfl_xor(mx, 16, WAVE));
-            mx = fmaxf(mx, __shfl_xor(mx, 32, WAVE)) * c2;
-            const float m2 = fmaxf(m[n], mx), keep = m[n] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m[n] - m2), neg = m2 == -INFINITY ? 0.f : -m2;
-            l[n] *= keep;
-#pragma unroll
-            for (int t = 0; t < NT; ++t)
-#pragma unroll
-                for (int r = 0; r < 4; ++r) o[n][t][r] *= keep;
-            m[n] = m2;
-            float e[8];
-#pragma unroll
-            for (int t = 0; t < 2; ++t)
-#pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    e[4 * t + r] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[n][t][r], c2, neg));
-                    l[n] += e[4 * t + r];
-                }
-            pf[n] = (u32x4_t){pack_bf(e[0], e[1]), pack_bf(e[2], e[3]), pack_bf(e[4], e[5]), pack_bf(e[6], e[7])};
         }
+        if (edge || first_step) raise();  // (elsewhere m is a reference, not a maximum: see block_role's step)
+        first_step = false;
+        u32x4_t pf[NQ];
+        float sum[NQ];
+        auto weights = [&]() {
+            const bf16x2_t one = {(__bf16)1.f, (__bf16)1.f};
+            bool over = false;
+#pragma unroll
+            for (int n = 0; n < NQ; ++n) {
+                const float neg = m[n] == -INFINITY ? 0.f : -m[n];
+                sum[n] = 0.f;
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                    const int t = q >> 1, r = 2 * (q & 1);
+                    const uint32_t pair = pack_bf(__builtin_amdgcn_exp2f(__builtin_fmaf(sc[n][t][r], c2, neg)), __builtin_amdgcn_exp2f(__builtin_fmaf(sc[n][t][r + 1], c2, neg)));
+                    pf[n][q] = pair;
+                    sum[n] = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2_t, pair), one, sum[n], false);
+                }
+                over |= !(sum[n] <= 0x1p60f);
+            }
+            return __any(over);
+        };
+        if (weights()) {
+            raise();
+            (void)weights();
+        }
+#pragma unroll
+        for (int n = 0; n < NQ; ++n) l[n] += sum[n];
         if (edge) {
             bool ill = false;  // inf or NaN among the values of a step that not every column sees whole
 #pragma unroll 1
@@ -744,12 +582,6 @@ __global__ __launch_bounds__(256) void prefix_attn_join_kernel(isst_prefix_attn 
 #ifndef PA_TAU
 #define PA_TAU 1.25
 #endif
-#ifndef PA_WIDE
-#define PA_WIDE 512
-#endif
-#ifndef PW_TAU
-#define PW_TAU 1.8
-#endif
 #ifndef PA_FIX
 #define PA_FIX 5.0
 #endif
@@ -782,19 +614,17 @@ static PrefixPlan plan(const isst_prefix_attn& a) {
     }
     if (a.prefix_len > 0) {
         p.prefix_block = cols > 32;
-        p.prefix_wide = cols >= PA_WIDE;
-        p.prefix_tiles = p.prefix_wide ? ceil_div(cols, 256) : p.prefix_block ? ceil_div(cols, width) : 1;
+        p.prefix_tiles = p.prefix_block ? ceil_div(cols, width) : 1;
         if (p.prefix_block) {
             // key spans: the rounds of the chip that the units take (with the own keys' units filling what a last round leaves) + what their partial results cost
-            const double tau = p.prefix_wide ? PW_TAU : PA_TAU, slots_now = p.prefix_wide ? 256 : room;
-            const int tiles = ceil_div(a.prefix_len, p.prefix_wide ? PW_TILE : PA_TILE), groups = a.kv_heads * p.prefix_tiles;
+            const int tiles = ceil_div(a.prefix_len, PA_TILE), groups = a.kv_heads * p.prefix_tiles;
             double best = 1e30;
             for (int s = 1; s <= PA_MAX_SLOTS - 8 && s <= tiles; ++s) {
                 const int per = ceil_div(tiles, s);
                 if (ceil_div(tiles, per) != s) continue;
-                const double dur = per * tau * (a.head_dim / 128.0) + PA_FIX, units = (double)groups * s;
-                const double even = (units * dur + own_us) / slots_now, rounds = dur * ceil_div((long)units, (long)slots_now);
-                const double t = (even > rounds && !p.prefix_wide ? even : rounds) + s * (double)a.rows * a.heads * (8.0 * a.head_dim) / 3e6;
+                const double dur = per * PA_TAU * (a.head_dim / 128.0) + PA_FIX, units = (double)groups * s;
+                const double even = (units * dur + own_us) / room, rounds = dur * ceil_div((long)units, (long)room);
+                const double t = (even > rounds ? even : rounds) + s * (double)a.rows * a.heads * (8.0 * a.head_dim) / 3e6;
                 if (t < best) { best = t; p.prefix_splits = s; }
             }
         } else {
@@ -819,11 +649,6 @@ int launch_prefix_attention(const isst_prefix_attn& a, void* workspace, hipStrea
     p.o = static_cast<float*>(workspace);
     p.ml = reinterpret_cast<float2*>(p.o + p.slots * pairs * a.head_dim);
     const int nq = span_nq(a);
-    if (p.prefix_wide) {
-        if (a.head_dim == 128) hipLaunchKernelGGL(prefix_attn_wide_kernel<128>, dim3((unsigned)p.prefix_units), dim3(256), 0, s, a, p);
-        else hipLaunchKernelGGL(prefix_attn_wide_kernel<64>, dim3((unsigned)p.prefix_units), dim3(256), 0, s, a, p);
-        p.prefix_units = 0;
-    }
     if (p.prefix_units + p.own_units > 0) {
         if (a.head_dim == 128) { if (nq == 1) launch_partial<128, 1>(a, p, s); else launch_partial<128, 2>(a, p, s); }
         else { if (nq == 1) launch_partial<64, 1>(a, p, s); else launch_partial<64, 2>(a, p, s); }
