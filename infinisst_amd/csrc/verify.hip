@@ -2,9 +2,9 @@
 // p, q = softmax of fp32 score rows.  Everything behind the scores is in 64 bits: the outcome of a comparison or of a draw must not depend on the order of a sum, and with
 // 32-bit probabilities the borders of the inverse CDF move by ~1e-8 each -- over 128 k of them one draw in a thousand would land elsewhere.
 //
-// Launch 1 reads every score row once, a workgroup per slice of VF_SLICE entries (maximum, its first index, sum of exponentials); its floor is that read, and the 64-bit exponential (~20
-// instructions) is short enough to hide behind it.  Launch 2 runs only where drafts bring scores: it sums what a refused draft leaves over, slice by slice.  Launch 3 takes one workgroup
-// per stream: decide, find the slice that the draw falls into from the slice sums, walk that slice.
+// Launch 1 reads every score row once, a workgroup per slice of VF_SLICE entries (maximum and its first index, or sum of exponentials); its floor is that read, and the 64-bit exponential
+// is short enough to hide most of itself behind it.  Drafts with scores need two more: who decides (a workgroup per stream), and what a refused draft leaves over, slice by slice.  The last
+// launch takes one workgroup per stream: find the slice that the draw falls into from the slice sums, walk that slice.
 #include "common.h"
 #include "kernels.h"
 
@@ -17,48 +17,89 @@ struct VerifyStat { double sum; float max; int at; };  // of a slice: sum of exp
 
 typedef float f32x4u_t __attribute__((ext_vector_type(4), aligned(4)));  // (rows start anywhere)
 
-// exp(d) for d <= 0: 2^k exp(r) with |r| <= ln 2 / 2 and the Taylor series up to r^11 / 11!, whose remainder is below 7e-15 relative.  NaN (-inf less -inf) and anything under -800: 0
-__device__ __forceinline__ double exp_le0(double d) {
-    d = fmax(d, -800.0);
-    const double k = rint(d * 1.4426950408889634074);
-    const double r = fma(-k, 0x1.abc9e3b39803fp-56, fma(-k, 0x1.62e42fefa39efp-1, d));  // ln 2 and what its rounding left
-    double p = 1.0 / 39916800.0;
-    p = fma(p, r, 1.0 / 3628800.0); p = fma(p, r, 1.0 / 362880.0); p = fma(p, r, 1.0 / 40320.0); p = fma(p, r, 1.0 / 5040.0); p = fma(p, r, 1.0 / 720.0);
-    p = fma(p, r, 1.0 / 120.0); p = fma(p, r, 1.0 / 24.0); p = fma(p, r, 1.0 / 6.0); p = fma(p, r, 0.5); p = fma(p, r, 1.0); p = fma(p, r, 1.0);
-    return ldexp(p, (int)k);
+// exp(d) for -700 <= d <= 0: 2^k exp(r), k the nearest whole number to d / ln 2 (added to 1.5 2^52, where it is the low word), |r| <= ln 2 / 2, the Taylor series up to r^10 / 10!.  Its
+// remainder is below 2.2e-13 relative: over 128 k borders of an inverse CDF one draw in 10^7 could land elsewhere for it.  17 instructions, 16 of them in 64 bits.
+__device__ __forceinline__ double exp_core(double d) {
+    const double t = fma(d, 1.4426950408889634074, 0x1.8p52), k = t - 0x1.8p52, r = fma(-k, 0.69314718055994530942, d);
+    double p = 1.0 / 3628800.0;
+    p = fma(p, r, 1.0 / 362880.0); p = fma(p, r, 1.0 / 40320.0); p = fma(p, r, 1.0 / 5040.0); p = fma(p, r, 1.0 / 720.0); p = fma(p, r, 1.0 / 120.0);
+    p = fma(p, r, 1.0 / 24.0); p = fma(p, r, 1.0 / 6.0); p = fma(p, r, 0.5); p = fma(p, r, 1.0); p = fma(p, r, 1.0);
+    return __hiloint2double(__double2hiint(p) + (__double2loint(t) << 20), __double2loint(p));
 }
-__device__ __forceinline__ double shfl_d(double v, int lane) {
-    const unsigned long long u = __double_as_longlong(v);
-    return __longlong_as_double(((unsigned long long)(unsigned)__shfl((int)(u >> 32), lane, WAVE) << 32) | (unsigned)__shfl((int)u, lane, WAVE));
+// ... for any d <= 0; under -700 and for NaN (-inf less -inf): 0
+__device__ __forceinline__ double exp_le0(double d) { return d >= -700.0 ? exp_core(d) : 0.0; }
+// 64-bit reductions over lanes on DPP (as common.h's 32-bit ones): the rows of 16 lanes inside the vector ALU, the four rows by v_readlane -- a tree of ds_bpermute pairs is 0.7 us of latency
+template <int CTRL>
+__device__ __forceinline__ double dpp_d(double v) {  // (lanes without a source: 0)
+    const int lo = __builtin_amdgcn_update_dpp(0, __double2loint(v), CTRL, 0xf, 0xf, true), hi = __builtin_amdgcn_update_dpp(0, __double2hiint(v), CTRL, 0xf, 0xf, true);
+    return __hiloint2double(hi, lo);
+}
+__device__ __forceinline__ double lane_d(double v, int lane) {
+    return __hiloint2double(__builtin_amdgcn_readlane(__double2hiint(v), lane), __builtin_amdgcn_readlane(__double2loint(v), lane));
+}
+__device__ __forceinline__ double row_sum_d(double v) {  // of the 16 lanes of a row, in each of them
+    v += dpp_d<0xb1>(v);
+    v += dpp_d<0x4e>(v);
+    v += dpp_d<0x124>(v);
+    v += dpp_d<0x128>(v);
+    return v;
+}
+__device__ __forceinline__ double half_sum_d(double v) {  // of the 32 lanes of a half wave
+    v = row_sum_d(v);
+    const double a = lane_d(v, 0) + lane_d(v, 16), b = lane_d(v, 32) + lane_d(v, 48);
+    return (threadIdx.x & 32) ? b : a;
 }
 __device__ __forceinline__ double wave_sum_d(double v) {
-#pragma unroll
-    for (int m = 1; m < 64; m <<= 1) v += shfl_d(v, (threadIdx.x & 63) ^ m);
-    return v;
+    v = row_sum_d(v);
+    return (lane_d(v, 0) + lane_d(v, 16)) + (lane_d(v, 32) + lane_d(v, 48));
 }
 // sum over this lane and the lanes before it
 __device__ __forceinline__ double wave_scan_d(double v) {
-#pragma unroll
-    for (int m = 1; m < 64; m <<= 1) {
-        const double o = shfl_d(v, (threadIdx.x & 63) - m);
-        if ((int)(threadIdx.x & 63) >= m) v += o;
-    }
-    return v;
+    v += dpp_d<0x111>(v);
+    v += dpp_d<0x112>(v);
+    v += dpp_d<0x114>(v);
+    v += dpp_d<0x118>(v);
+    const double r0 = lane_d(v, 15), r1 = r0 + lane_d(v, 31), r2 = r1 + lane_d(v, 47);
+    const int row = (threadIdx.x & 63) >> 4;
+    return row == 0 ? v : v + (row == 1 ? r0 : row == 2 ? r1 : r2);
+}
+// the (value, lowest index) maximum of the 32 lanes of a half wave
+__device__ __forceinline__ void half_argmax(float& m, int& at) {
+    float v = m;
+    v = fmaxf(v, __int_as_float(dpp_take<0xb1>(__float_as_int(v))));
+    v = fmaxf(v, __int_as_float(dpp_take<0x4e>(__float_as_int(v))));
+    v = fmaxf(v, __int_as_float(dpp_take<0x124>(__float_as_int(v))));
+    v = fmaxf(v, __int_as_float(dpp_take<0x128>(__float_as_int(v))));
+    auto lane_f = [&](int l) { return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), l)); };
+    const float a = fmaxf(lane_f(0), lane_f(16)), b = fmaxf(lane_f(32), lane_f(48));
+    v = (threadIdx.x & 32) ? b : a;
+    int i = m == v ? at : 0x7fffffff;
+    i = min(i, dpp_take<0xb1>(i));
+    i = min(i, dpp_take<0x4e>(i));
+    i = min(i, dpp_take<0x124>(i));
+    i = min(i, dpp_take<0x128>(i));
+    const int ia = min(__builtin_amdgcn_readlane(i, 0), __builtin_amdgcn_readlane(i, 16)), ib = min(__builtin_amdgcn_readlane(i, 32), __builtin_amdgcn_readlane(i, 48));
+    m = v;
+    at = (threadIdx.x & 32) ? ib : ia;
 }
 __device__ __forceinline__ int slices(int vocab) { return (vocab + VF_SLICE - 1) / VF_SLICE; }
 __device__ __forceinline__ int rows_of(const VerifyArgs& g) { return g.max_drafts + 1 + (g.draft ? g.max_drafts : 0); }
 __device__ __forceinline__ const VerifyStat* stats_of(const VerifyArgs& g, int b, int row) {
     return static_cast<const VerifyStat*>(g.workspace) + ((long)b * rows_of(g) + row) * slices(g.vocab);
 }
-__device__ __forceinline__ double* left_of(const VerifyArgs& g, int b) {  // launch 2's slice sums
-    return reinterpret_cast<double*>(static_cast<VerifyStat*>(g.workspace) + (long)g.streams * rows_of(g) * slices(g.vocab)) + (long)b * slices(g.vocab);
+// behind the statistics, per stream: what a refused draft with scores leaves over, [slices]; or, of drafts without, the sum of the draft's slice without the draft, [max_drafts]
+__device__ __forceinline__ int rest_of(const VerifyArgs& g) { return g.draft ? slices(g.vocab) : g.max_drafts; }
+__device__ __forceinline__ double* left_of(const VerifyArgs& g, int b) {
+    return reinterpret_cast<double*>(static_cast<VerifyStat*>(g.workspace) + (long)g.streams * rows_of(g) * slices(g.vocab)) + (long)b * rest_of(g);
 }
 __device__ __forceinline__ const float* target_row(const VerifyArgs& g, int b, int i) { return g.target + b * g.target_stream + i * g.target_row; }
 __device__ __forceinline__ const float* draft_row(const VerifyArgs& g, int b, int i) { return g.draft + b * g.draft_stream + i * g.draft_row; }
 
 // grid (slices, score rows)
+template <bool GREEDY>
 __global__ __launch_bounds__(VF_THREADS) void verify_stats_kernel(VerifyArgs g) {
     __shared__ VerifyStat part[VF_THREADS / 64];
+    __shared__ double rests[VF_THREADS / 64];
     const int tid = threadIdx.x, wave = tid >> 6, rows_t = g.max_drafts + 1, per = rows_of(g);
     const int b = blockIdx.y / per, i = blockIdx.y % per, lo = blockIdx.x * VF_SLICE;
     const float* x = i < rows_t ? target_row(g, b, i) : draft_row(g, b, i - rows_t);
@@ -82,40 +123,57 @@ __global__ __launch_bounds__(VF_THREADS) void verify_stats_kernel(VerifyArgs g) 
 #pragma unroll
     for (int k = 0; k < VF_PER; ++k) {
         bad |= !(s[k] < INFINITY);  // NaN or +inf
-        if (s[k] > m) { m = s[k]; at = lo + ((k >> 2) * VF_THREADS + tid) * 4 + (k & 3); }
+        if (!GREEDY) m = fmaxf(m, s[k]);
+        else if (s[k] > m) { m = s[k]; at = lo + ((k >> 2) * VF_THREADS + tid) * 4 + (k & 3); }
     }
-    wave_argmax_all(m, at);
-    double sum = 0.0;
-    if (g.uniforms) {
+    double sum = 0.0, rest = 0.0;
+    int x_at = -1;  // the row's draft, where it comes without scores and lies in this slice
+    if constexpr (GREEDY) {
+        wave_argmax_all(m, at);
+    } else {
+        m = wave_max_all(m);
 #pragma unroll
-        for (int k = 0; k < VF_PER; ++k) sum += exp_le0((double)s[k] - (double)m);
+        for (int k = 0; k < VF_PER; ++k) sum += exp_core(fmax((double)s[k] - (double)m, -700.0));  // (1e-304 for a removed entry: not one bit of a sum that is 1 or more)
         sum = wave_sum_d(sum);
+        if (!g.draft && i < g.max_drafts) {
+            const int xi = g.drafts[(long)b * g.max_drafts + i];
+            if (xi >= lo && xi - lo < VF_SLICE) x_at = xi;
+        }
+        if (x_at >= 0) {
+#pragma unroll
+            for (int k = 0; k < VF_PER; ++k) rest += lo + ((k >> 2) * VF_THREADS + tid) * 4 + (k & 3) == x_at ? 0.0 : exp_le0((double)s[k] - (double)m);
+            rest = wave_sum_d(rest);
+        }
     }
     bad = __any(bad);
-    if ((tid & 63) == 0) part[wave] = {sum, bad ? NAN : m, at};
+    if ((tid & 63) == 0) { part[wave] = {sum, bad ? NAN : m, at}; rests[wave] = rest; }
     __syncthreads();
     if (tid == 0) {
         VerifyStat t = part[0];
+        double r = rests[0];
         for (int w = 1; w < VF_THREADS / 64; ++w) {
             const VerifyStat o = part[w];
             if (!(t.max == t.max) || !(o.max == o.max)) { t.max = NAN; continue; }
             const float M = fmaxf(t.max, o.max);
-            t.sum = t.sum * exp_le0((double)t.max - (double)M) + o.sum * exp_le0((double)o.max - (double)M);
+            const double et = exp_le0((double)t.max - (double)M), eo = exp_le0((double)o.max - (double)M);
+            t.sum = t.sum * et + o.sum * eo;
+            r = r * et + rests[w] * eo;
             if (o.max > t.max) t.at = o.at;  // (equal: the lower index is the earlier one -- below)
             else if (o.max == t.max) t.at = min(t.at, o.at);
             t.max = M;
         }
         static_cast<VerifyStat*>(g.workspace)[(long)blockIdx.y * gridDim.x + blockIdx.x] = t;
+        if (x_at >= 0) left_of(g, b)[i] = r;
     }
 }
 
-// one row's statistics from its slices, by one wave, in every lane; max = NaN: no distribution
+// one row's statistics from its slices, by the 32 lanes of a half wave (row < 0: none of its business), in each of them; max = NaN: no distribution
 __device__ __forceinline__ VerifyStat merge_row(const VerifyArgs& g, int b, int row) {
-    const VerifyStat* st = stats_of(g, b, row);
-    const int S = slices(g.vocab), lane = threadIdx.x & 63;
+    const VerifyStat* st = stats_of(g, b, max(row, 0));
+    const int S = row < 0 ? 0 : slices(g.vocab), lane = threadIdx.x & 31;
     VerifyStat t = {0.0, -INFINITY, 0x7fffffff};
     bool bad = false;
-    for (int s = lane; s < S; s += 64) {
+    for (int s = lane; s < S; s += 32) {
         const VerifyStat o = st[s];
         bad |= !(o.max == o.max);
         const float M = fmaxf(t.max, o.max);
@@ -125,9 +183,10 @@ __device__ __forceinline__ VerifyStat merge_row(const VerifyArgs& g, int b, int 
     }
     float M = t.max;
     int at = t.at;
-    wave_argmax_all(M, at);
-    t.sum = wave_sum_d(t.sum * exp_le0((double)t.max - (double)M));
-    t.max = __any(bad) || M == -INFINITY ? NAN : M;
+    half_argmax(M, at);
+    t.sum = half_sum_d(t.sum * exp_le0((double)t.max - (double)M));
+    const unsigned long long bads = __ballot(bad);
+    t.max = ((threadIdx.x & 32) ? bads >> 32 : bads & 0xffffffffull) || M == -INFINITY ? NAN : M;
     t.at = at;
     return t;
 }
@@ -148,13 +207,13 @@ __device__ __forceinline__ Decision decide(const VerifyArgs& g, int b) {
     if (d.n < 0 || d.n > K) return d;
     for (int i0 = 0;; i0 += VF_ROWS) {
         const int cnt = min(VF_ROWS, d.n - i0);  // drafts of this turn; the row behind the last one is looked at as well
-        for (int k = wave; k < 2 * cnt + 1; k += VF_THREADS / 64) {
-            if (k <= cnt) {
-                const VerifyStat t = merge_row(g, b, i0 + k);
-                if ((tid & 63) == 0) sp[k] = t;
-            } else if (g.draft) {
-                const VerifyStat t = merge_row(g, b, K + 1 + i0 + k - cnt - 1);
-                if ((tid & 63) == 0) sq[k - cnt - 1] = t;
+        const int looks = g.draft ? 2 * cnt + 1 : cnt + 1;
+        for (int k0 = 2 * wave; k0 < looks; k0 += VF_THREADS / 32) {
+            const int k = k0 + ((tid >> 5) & 1);
+            const VerifyStat t = merge_row(g, b, k >= looks ? -1 : k <= cnt ? i0 + k : K + 1 + i0 + k - cnt - 1);
+            if ((tid & 31) == 0 && k < looks) {
+                if (k <= cnt) sp[k] = t;
+                else sq[k - cnt - 1] = t;
             }
         }
         if (tid == 0) s_stop = cnt;
@@ -253,20 +312,27 @@ __device__ __forceinline__ double slice_sum(const VerifyArgs& g, int b, const De
     return total;
 }
 
+__device__ __forceinline__ Decision* decision_of(const VerifyArgs& g, int b) { return reinterpret_cast<Decision*>(left_of(g, g.streams)) + b; }
+__global__ __launch_bounds__(VF_THREADS) void verify_decide_kernel(VerifyArgs g) {
+    const Decision d = decide(g, blockIdx.x);
+    if (threadIdx.x == 0) *decision_of(g, blockIdx.x) = d;
+}
+
 // grid (slices, streams): what a refused draft with scores leaves over
 __global__ __launch_bounds__(VF_THREADS) void verify_left_kernel(VerifyArgs g) {
-    const Decision d = decide(g, blockIdx.y);
+    const Decision d = *decision_of(g, blockIdx.y);
     if (d.accepted < 0 || d.accepted == d.n) return;
     const double s = slice_sum(g, blockIdx.y, d, 0, blockIdx.x * VF_SLICE);
     if (threadIdx.x == 0) left_of(g, blockIdx.y)[blockIdx.x] = s;
 }
 
 // one workgroup per stream
+template <bool DECIDED>
 __global__ __launch_bounds__(VF_THREADS) void verify_draw_kernel(VerifyArgs g) {
     __shared__ int s_slice, s_live, s_at, s_last;
     __shared__ double s_before, s_total;
     const int b = blockIdx.x, tid = threadIdx.x, K = g.max_drafts, S = slices(g.vocab);
-    const Decision d = decide(g, b);
+    const Decision d = DECIDED ? *decision_of(g, b) : decide(g, b);
     int pick = -1;
     bool bad = d.accepted < 0;
     if (!bad && !g.uniforms) pick = d.p.at;
@@ -275,23 +341,24 @@ __global__ __launch_bounds__(VF_THREADS) void verify_draw_kernel(VerifyArgs g) {
         bad = !(u >= 0.0 && u < 1.0);
         const VerifyStat* st = stats_of(g, b, d.accepted);
         for (int kind = bad ? 3 : d.accepted == d.n ? 2 : g.draft ? 0 : 1; kind < 3; kind = 2) {
-            const int xs = kind == 1 ? g.drafts[(long)b * K + d.accepted] / VF_SLICE : -1;  // (the slice that the draft is taken out of is summed anew)
-            const double without = kind == 1 ? slice_sum(g, b, d, 1, xs * VF_SLICE) : 0.0;
+            const int xs = kind == 1 ? g.drafts[(long)b * K + d.accepted] / VF_SLICE : -1;  // (the slice that the draft is taken out of)
             auto of_slice = [&](int s) {
-                return kind == 0 ? left_of(g, b)[s] : s == xs ? without : st[s].sum * exp_le0((double)st[s].max - (double)d.p.max) / d.p.sum;
+                if (kind == 0) return left_of(g, b)[s];
+                return (s == xs ? left_of(g, b)[d.accepted] : st[s].sum) * exp_le0((double)st[s].max - (double)d.p.max) / d.p.sum;
             };
             if (tid < 64) {  // total, then the slice whose running sum first exceeds u total (none, by rounding: the last one that holds anything)
                 double total = 0.0;
-                for (int s0 = 0; s0 < S; s0 += 64) total += wave_sum_d(s0 + tid < S ? of_slice(s0 + tid) : 0.0);
+                const double head = tid < S ? of_slice(tid) : 0.0;
+                for (int s0 = 0; s0 < S; s0 += 64) total += wave_sum_d(s0 == 0 ? head : s0 + tid < S ? of_slice(s0 + tid) : 0.0);
                 int slice = -1, live = -1;
                 double before = 0.0, cum = 0.0;
                 for (int s0 = 0; s0 < S && slice < 0; s0 += 64) {
-                    const double v = s0 + tid < S ? of_slice(s0 + tid) : 0.0, c = cum + wave_scan_d(v);
+                    const double v = s0 == 0 ? head : s0 + tid < S ? of_slice(s0 + tid) : 0.0, c = cum + wave_scan_d(v);
                     const unsigned long long hit = __ballot(v > 0.0 && c > u * total), any = __ballot(v > 0.0);
                     const int at = hit ? __builtin_ctzll(hit) : any ? 63 - __builtin_clzll(any) : -1;
-                    if (at >= 0) { live = s0 + at; before = shfl_d(c - v, at); }
+                    if (at >= 0) { live = s0 + at; before = lane_d(c - v, __builtin_amdgcn_readfirstlane(at)); }
                     if (hit) slice = live;
-                    cum = shfl_d(c, 63);
+                    cum = lane_d(c, 63);
                 }
                 if (tid == 0) { s_slice = slice; s_live = live; s_before = before; s_total = total; s_at = 0x7fffffff; s_last = -1; }
             }
@@ -330,7 +397,8 @@ __global__ __launch_bounds__(VF_THREADS) void verify_draw_kernel(VerifyArgs g) {
 
 static int64_t n_slices(int vocab) { return ((int64_t)vocab + VF_SLICE - 1) / VF_SLICE; }
 int64_t verify_workspace(int streams, int max_drafts, int vocab) {
-    return streams * n_slices(vocab) * ((2 * (int64_t)max_drafts + 1) * (int64_t)sizeof(VerifyStat) + (int64_t)sizeof(double));
+    const int64_t rest = n_slices(vocab) > max_drafts ? n_slices(vocab) : max_drafts;
+    return streams * (n_slices(vocab) * (2 * (int64_t)max_drafts + 1) * (int64_t)sizeof(VerifyStat) + rest * (int64_t)sizeof(double) + (int64_t)sizeof(Decision));
 }
 int launch_verify(const VerifyArgs& g, hipStream_t s) {
     const int64_t S = n_slices(g.vocab);
@@ -348,9 +416,16 @@ int launch_verify(const VerifyArgs& g, hipStream_t s) {
         t.tokens += (int64_t)b0 * (g.max_drafts + 1);
         t.counts += b0;
         t.workspace = static_cast<char*>(g.workspace) + verify_workspace(b0, g.max_drafts, g.vocab);
-        hipLaunchKernelGGL(verify_stats_kernel, dim3((unsigned)S, (unsigned)(t.streams * per)), dim3(VF_THREADS), 0, s, t);
-        if (t.draft && t.uniforms) hipLaunchKernelGGL(verify_left_kernel, dim3((unsigned)S, (unsigned)t.streams), dim3(VF_THREADS), 0, s, t);
-        hipLaunchKernelGGL(verify_draw_kernel, dim3((unsigned)t.streams), dim3(VF_THREADS), 0, s, t);
+        const dim3 grid((unsigned)S, (unsigned)(t.streams * per)), block(VF_THREADS), per_stream((unsigned)t.streams);
+        if (!t.uniforms) hipLaunchKernelGGL(verify_stats_kernel<true>, grid, block, 0, s, t);
+        else hipLaunchKernelGGL(verify_stats_kernel<false>, grid, block, 0, s, t);
+        if (t.draft) {
+            hipLaunchKernelGGL(verify_decide_kernel, per_stream, block, 0, s, t);
+            hipLaunchKernelGGL(verify_left_kernel, dim3((unsigned)S, (unsigned)t.streams), block, 0, s, t);
+            hipLaunchKernelGGL(verify_draw_kernel<true>, per_stream, block, 0, s, t);
+        } else {
+            hipLaunchKernelGGL(verify_draw_kernel<false>, per_stream, block, 0, s, t);
+        }
     }
     return hipGetLastError() == hipSuccess ? ISST_OK : ISST_ERR_HIP;
 }
