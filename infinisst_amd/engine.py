@@ -797,12 +797,13 @@ def op_prefix_attention(q: torch.Tensor, k_prefix: torch.Tensor, v_prefix: torch
     bf = torch.bfloat16
     (rows, heads, D), (kv, P, _), (seqs, _, cap, _) = q.shape, k_prefix.shape, k_tail.shape
     prefix, tail = (kv, P, D), (seqs, kv, cap, D)
-    _expect(what, dev, "q", q, bf, (rows, heads, D), False)
-    _expect(what, dev, "k_prefix", k_prefix, bf, prefix, False)
-    _expect(what, dev, "v_prefix", v_prefix, bf, prefix, False)
-    _expect(what, dev, "k_tail", k_tail, bf, tail, False)
-    _expect(what, dev, "v_tail", v_tail, bf, tail, False)
-    _expect(what, dev, "tail_lens", tail_lens, torch.int32, (seqs,))
+    if not (q.dtype is bf and k_prefix.dtype is bf and v_prefix.dtype is bf and k_tail.dtype is bf and v_tail.dtype is bf and tail_lens.dtype is torch.int32
+            and v_prefix.shape == prefix and k_prefix.shape == prefix and k_tail.shape == tail and v_tail.shape == tail and tail_lens.shape == (seqs,)
+            and k_prefix.get_device() == dev and v_prefix.get_device() == dev and k_tail.get_device() == dev and v_tail.get_device() == dev
+            and tail_lens.get_device() == dev and tail_lens.is_contiguous()):
+        for name, t, shape in (("q", q, q.shape), ("k_prefix", k_prefix, prefix), ("v_prefix", v_prefix, prefix), ("k_tail", k_tail, tail), ("v_tail", v_tail, tail)):
+            _expect(what, dev, name, t, bf, shape, False)
+        _expect(what, dev, "tail_lens", tail_lens, torch.int32, (seqs,))
     if row_starts is not None:
         _expect(what, dev, "row_starts", row_starts, torch.int32, (seqs + 1,))
     if out is None:
