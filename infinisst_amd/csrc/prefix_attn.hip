@@ -17,6 +17,7 @@ typedef __attribute__((ext_vector_type(16))) float f32x16_t;
 typedef __attribute__((ext_vector_type(4))) short s16x4_t;
 
 #define PA_TILE 32               // keys of a block tile
+#define PA_RAISE 0x1p16f         // sum of a step's weights from which a column's reference exponent is raised
 // Keys and values are read through buffer descriptors that start at a tile's first row: a lane's offset is either its row's (rows lie up to 2^25 bytes apart, 63 of them stay inside the
 // descriptor) or PA_OOB, for which the load returns zeros -- also with the scalar offset of the row group added.
 #define PA_EXTENT 0x7fffffffu
@@ -188,8 +189,7 @@ __device__ __forceinline__ void block_role(const isst_prefix_attn& a, const Pref
         m = m2;
     };
     // weights of the tile (bf16 pairs in the layout of the value product) and their sum in this lane, as the product will see them
-    auto weights = [&](u32x4_t (&pf)[2]) {
-        const float neg = m == -INFINITY ? 0.f : -m;
+    auto weights = [&](u32x4_t (&pf)[2], float neg) {
         const bf16x2_t one = {(__bf16)1.f, (__bf16)1.f};
         float sum = 0.f;
 #pragma unroll
@@ -205,7 +205,7 @@ __device__ __forceinline__ void block_role(const isst_prefix_attn& a, const Pref
     };
     // One tile: its scores are in sc, those of the next are computed on the way.  EDGE: some column does not see some key of it.
     // A column's reference m is the maximum of its first tile (and of its edge tiles): weights are exponentials against it, bf16 and fp32 hold them to 2^127, and no bit is lost by their
-    // size.  So other maxima are not looked for -- that and the running sum were 100 of the 169 vector instructions of a tile -- and only weights that pass 2^60 (or NaN) move m,
+    // size.  So other maxima are not looked for -- that and the running sum were 100 of the 169 vector instructions of a tile -- and only weights that pass PA_RAISE (or NaN) move m,
     // before anything of the tile was used.
     auto step = [&](int i, auto edge) {
         constexpr bool EDGE = decltype(edge)::value;
@@ -228,11 +228,12 @@ __device__ __forceinline__ void block_role(const isst_prefix_attn& a, const Pref
             ill = __any(ill);
         }
         u32x4_t pf[2];
-        float sum = weights(pf);
+        auto at = [&]() { return m == -INFINITY ? 0.f : -m; };
+        float sum = weights(pf, EDGE ? at() : -m);  // (no reference yet, all scores so far -inf: weights of inf, or NaN, which set one)
         if constexpr (!EDGE)
-            if (__any(!(sum <= 0x1p60f))) {
+            if (__any(!(sum <= PA_RAISE))) {
                 raise();
-                sum = weights(pf);
+                sum = weights(pf, at());
             }
         l += sum;
         const f32x16_t sn = scores(next);
@@ -398,12 +399,12 @@ __device__ __forceinline__ void span_role(const isst_prefix_attn& a, const Prefi
         first_step = false;
         u32x4_t pf[NQ];
         float sum[NQ];
-        auto weights = [&]() {
+        auto weights = [&](float none) {  // none: what a column without a reference subtracts (inf: its weights come out as inf or NaN, and set one)
             const bf16x2_t one = {(__bf16)1.f, (__bf16)1.f};
             bool over = false;
 #pragma unroll
             for (int n = 0; n < NQ; ++n) {
-                const float neg = m[n] == -INFINITY ? 0.f : -m[n];
+                const float neg = m[n] == -INFINITY ? none : -m[n];
                 sum[n] = 0.f;
 #pragma unroll
                 for (int q = 0; q < 4; ++q) {
@@ -412,13 +413,13 @@ __device__ __forceinline__ void span_role(const isst_prefix_attn& a, const Prefi
                     pf[n][q] = pair;
                     sum[n] = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2_t, pair), one, sum[n], false);
                 }
-                over |= !(sum[n] <= 0x1p60f);
+                over |= !(sum[n] <= PA_RAISE);
             }
             return __any(over);
         };
-        if (weights()) {
+        if (weights(INFINITY)) {
             raise();
-            (void)weights();
+            (void)weights(0.f);
         }
 #pragma unroll
         for (int n = 0; n < NQ; ++n) l[n] += sum[n];

@@ -183,6 +183,39 @@ def test_prefix_attention_large_scores():
         assert bool(((got - o).abs() <= tol).all())
 
 
+@pytest.mark.parametrize("rows,D", [([1, 2], 128), ([40, 33], 128), ([1] * 40, 64)])
+@pytest.mark.parametrize("removed", [-math.inf, -3.3895313892515355e38])
+def test_prefix_attention_scores_of_minus_infinity(rows, D, removed):
+    """Keys whose scores are -inf (whole tiles of them, at the start of the prefix, of a span and of the own keys) leave the other keys' weights as they are, also where those are far below zero."""
+    H, KV, P, cap = 4, 1, 700, 300
+    lens = [n + 200 for n in rows]
+    q, kp, vp, kt, vt, ln, st = attn_inputs(21, rows, lens, H, KV, D, P, cap)
+    q[..., 0], q[..., 1] = 4.0, 64.0
+    kp[..., 1], kt[:, :, :, 1] = -32.0, -32.0  # scores around -2048 / sqrt(D)
+    kp[..., 0], kt[..., 0] = 0.0, 0.0
+    kp[:, :170, 0] = kp[:, 300:420, 0] = kt[:, :, :130, 0] = removed
+    kp[..., 0, 0] = removed
+    o, A = attn_ref(q, kp, vp, kt, vt, ln, st)
+    assert bool(torch.isfinite(o).all())
+    got = E.op_prefix_attention(q, kp, vp, kt, vt, ln, st, max(rows)).cpu().double()
+    # sum |q k| scale is 2048 / sqrt(D) here, not 20: its rounding, 2^-24 D of it, is below 2^-8
+    tol = U_BF * o.abs() + (U_BF + 2.0 * 2.0 ** -24 * D * 2300 / math.sqrt(D)) * A
+    assert bool(((got - o).abs() <= tol).all())
+
+
+def test_prefix_attention_scores_that_grow():
+    """Scores that rise by hundreds from the first keys on: every reference that a column starts with is far below its maximum."""
+    rows, lens, H, KV, D, P, cap = [3, 30], [90, 200], 4, 2, 128, 900, 256
+    q, kp, vp, kt, vt, ln, st = attn_inputs(23, rows, lens, H, KV, D, P, cap)
+    q[..., 0] = 8.0
+    kp[..., 0] = (torch.arange(P, device=DEV) * 0.5).to(BF)  # up to 8 * 450 / sqrt(128) = 318
+    kt[..., 0] = (400 - torch.arange(cap, device=DEV)).to(BF)
+    o, A = attn_ref(q, kp, vp, kt, vt, ln, st)
+    got = E.op_prefix_attention(q, kp, vp, kt, vt, ln, st, 30).cpu().double()
+    tol = U_BF * o.abs() + (U_BF + 2.0 * 2.0 ** -24 * D * 340) * A
+    assert bool(((got - o).abs() <= tol).all())
+
+
 def test_prefix_attention_offsets_past_32_bits():
     rows, lens, H, KV, D, P, cap = [1, 2], [40, 41], 4, 2, 128, 150, 48
     q, kp, vp, kt, vt, ln, st = attn_inputs(13, rows, lens, H, KV, D, P, cap)
