@@ -102,6 +102,7 @@ __global__ __launch_bounds__(VF_THREADS) void verify_stats_kernel(VerifyArgs g) 
     __shared__ double rests[VF_THREADS / 64];
     const int tid = threadIdx.x, wave = tid >> 6, rows_t = g.max_drafts + 1, per = rows_of(g);
     const int b = blockIdx.y / per, i = blockIdx.y % per, lo = blockIdx.x * VF_SLICE;
+    if (g.n_drafts && (i < rows_t ? i : i - rows_t + 1) > g.n_drafts[b]) return;  // (a row behind the stream's drafts)
     const float* x = i < rows_t ? target_row(g, b, i) : draft_row(g, b, i - rows_t);
     float s[VF_PER];
     int bad = 0;
