@@ -12,6 +12,7 @@
 #define VF_PER 16                          // entries of a lane
 #define VF_SLICE (VF_THREADS * VF_PER)
 #define VF_ROWS 32                         // drafts that are decided at a time
+#define VF_DRAW 512                       // threads of the workgroup that decides and draws for a stream: its time is latency, and the walk through a slice takes eight exponentials a lane
 
 struct VerifyStat { double sum; float max; int at; };  // of a slice: sum of exp(score - max), max (NaN: a NaN or +inf among the scores), the maximum's first index
 
@@ -196,7 +197,7 @@ struct Decision {
     int accepted, n;  // accepted < 0: no answer
     VerifyStat p, q;  // of the row that decides (q: of the refused draft's scores)
 };
-// by the whole workgroup, the same in every thread
+// by the whole workgroup of VF_DRAW threads, the same in every thread
 __device__ __forceinline__ Decision decide(const VerifyArgs& g, int b) {
     __shared__ VerifyStat sp[VF_ROWS + 1], sq[VF_ROWS];
     __shared__ int s_stop, s_bad;
@@ -209,7 +210,7 @@ __device__ __forceinline__ Decision decide(const VerifyArgs& g, int b) {
     for (int i0 = 0;; i0 += VF_ROWS) {
         const int cnt = min(VF_ROWS, d.n - i0);  // drafts of this turn; the row behind the last one is looked at as well
         const int looks = g.draft ? 2 * cnt + 1 : cnt + 1;
-        for (int k0 = 2 * wave; k0 < looks; k0 += VF_THREADS / 32) {
+        for (int k0 = 2 * wave; k0 < looks; k0 += VF_DRAW / 32) {
             const int k = k0 + ((tid >> 5) & 1);
             const VerifyStat t = merge_row(g, b, k >= looks ? -1 : k <= cnt ? i0 + k : K + 1 + i0 + k - cnt - 1);
             if ((tid & 31) == 0 && k < looks) {
@@ -264,14 +265,15 @@ __device__ __forceinline__ double weight(int kind, const Decision& d, float t, f
     if (kind == 1) return is_draft ? 0.0 : p;
     return fmax(p - exp_le0((double)q - (double)d.q.max) * inv_q, 0.0);
 }
-// the lane's entries lo + VF_PER tid .. of the slice
-__device__ __forceinline__ void weights(const VerifyArgs& g, int b, const Decision& d, int kind, int lo, double (&w)[VF_PER]) {
-    const int i = d.accepted, v0 = lo + VF_PER * threadIdx.x, xi = kind == 1 ? g.drafts[(long)b * g.max_drafts + i] : -1;
+// the lane's entries lo + PER tid .. of the slice
+template <int PER>
+__device__ __forceinline__ void weights(const VerifyArgs& g, int b, const Decision& d, int kind, int lo, double (&w)[PER]) {
+    const int i = d.accepted, v0 = lo + PER * threadIdx.x, xi = kind == 1 ? g.drafts[(long)b * g.max_drafts + i] : -1;
     const float *t = target_row(g, b, i), *q = kind == 0 ? draft_row(g, b, i) : t;
     const double inv_p = 1.0 / d.p.sum, inv_q = kind == 0 ? 1.0 / d.q.sum : 0.0;
-    float ts[VF_PER], qs[VF_PER];
+    float ts[PER], qs[PER];
 #pragma unroll
-    for (int k = 0; k < VF_PER; k += 4) {
+    for (int k = 0; k < PER; k += 4) {
         if (v0 + k + 4 <= g.vocab) {
             const f32x4u_t f = *reinterpret_cast<const f32x4u_t*>(t + v0 + k), h = *reinterpret_cast<const f32x4u_t*>(q + v0 + k);
 #pragma unroll
@@ -285,11 +287,12 @@ __device__ __forceinline__ void weights(const VerifyArgs& g, int b, const Decisi
         }
     }
 #pragma unroll
-    for (int k = 0; k < VF_PER; ++k) w[k] = weight(kind, d, ts[k], qs[k], v0 + k == xi, inv_p, inv_q);
+    for (int k = 0; k < PER; ++k) w[k] = weight(kind, d, ts[k], qs[k], v0 + k == xi, inv_p, inv_q);
 }
 // inclusive sum over the workgroup's threads in thread order, and the total
+template <int THREADS>
 __device__ __forceinline__ double block_scan(double v, double& total) {
-    __shared__ double wsum[VF_THREADS / 64];
+    __shared__ double wsum[THREADS / 64];
     const int wave = threadIdx.x >> 6;
     v = wave_scan_d(v);
     __syncthreads();
@@ -298,7 +301,7 @@ __device__ __forceinline__ double block_scan(double v, double& total) {
     double before = 0.0;
     total = 0.0;
 #pragma unroll
-    for (int w = 0; w < VF_THREADS / 64; ++w) {
+    for (int w = 0; w < THREADS / 64; ++w) {
         if (w < wave) before += wsum[w];
         total += wsum[w];
     }
@@ -306,15 +309,15 @@ __device__ __forceinline__ double block_scan(double v, double& total) {
 }
 __device__ __forceinline__ double slice_sum(const VerifyArgs& g, int b, const Decision& d, int kind, int lo) {
     double w[VF_PER], mine = 0.0, total;
-    weights(g, b, d, kind, lo, w);
+    weights<VF_PER>(g, b, d, kind, lo, w);
 #pragma unroll
     for (int k = 0; k < VF_PER; ++k) mine += w[k];
-    block_scan(mine, total);
+    block_scan<VF_THREADS>(mine, total);
     return total;
 }
 
 __device__ __forceinline__ Decision* decision_of(const VerifyArgs& g, int b) { return reinterpret_cast<Decision*>(left_of(g, g.streams)) + b; }
-__global__ __launch_bounds__(VF_THREADS) void verify_decide_kernel(VerifyArgs g) {
+__global__ __launch_bounds__(VF_DRAW) void verify_decide_kernel(VerifyArgs g) {
     const Decision d = decide(g, blockIdx.x);
     if (threadIdx.x == 0) *decision_of(g, blockIdx.x) = d;
 }
@@ -329,8 +332,9 @@ __global__ __launch_bounds__(VF_THREADS) void verify_left_kernel(VerifyArgs g) {
 
 // one workgroup per stream
 template <bool DECIDED>
-__global__ __launch_bounds__(VF_THREADS) void verify_draw_kernel(VerifyArgs g) {
-    __shared__ int s_slice, s_live, s_at, s_last;
+__global__ __launch_bounds__(VF_DRAW) void verify_draw_kernel(VerifyArgs g) {
+    constexpr int PER = VF_SLICE / VF_DRAW;
+    __shared__ int s_slice, s_live, s_at[VF_DRAW / 64], s_last[VF_DRAW / 64];
     __shared__ double s_before, s_total;
     const int b = blockIdx.x, tid = threadIdx.x, K = g.max_drafts, S = slices(g.vocab);
     const Decision d = DECIDED ? *decision_of(g, b) : decide(g, b);
@@ -361,7 +365,7 @@ __global__ __launch_bounds__(VF_THREADS) void verify_draw_kernel(VerifyArgs g) {
                     if (hit) slice = live;
                     cum = lane_d(c, 63);
                 }
-                if (tid == 0) { s_slice = slice; s_live = live; s_before = before; s_total = total; s_at = 0x7fffffff; s_last = -1; }
+                if (tid == 0) { s_slice = slice; s_live = live; s_before = before; s_total = total; }
             }
             __syncthreads();
             const double total = s_total, goal = s_slice < 0 ? INFINITY : u * total;
@@ -371,28 +375,33 @@ __global__ __launch_bounds__(VF_THREADS) void verify_draw_kernel(VerifyArgs g) {
                 if (kind == 2) break;
                 continue;
             }
-            double w[VF_PER], mine = 0.0, all;
-            weights(g, b, d, kind, slice * VF_SLICE, w);
+            double w[PER], mine = 0.0, all;
+            weights<PER>(g, b, d, kind, slice * VF_SLICE, w);
 #pragma unroll
-            for (int k = 0; k < VF_PER; ++k) mine += w[k];
-            double cum = s_before + (block_scan(mine, all) - mine);
+            for (int k = 0; k < PER; ++k) mine += w[k];
+            double cum = s_before + (block_scan<VF_DRAW>(mine, all) - mine);
             int at = 0x7fffffff, last = -1;
 #pragma unroll
-            for (int k = 0; k < VF_PER; ++k) {
+            for (int k = 0; k < PER; ++k) {
                 if (!(w[k] > 0.0)) continue;
                 cum += w[k];
-                last = slice * VF_SLICE + VF_PER * tid + k;
+                last = slice * VF_SLICE + PER * tid + k;
                 if (cum > goal && at == 0x7fffffff) at = last;
             }
-            if (at != 0x7fffffff) atomicMin(&s_at, at);
-            if (last >= 0) atomicMax(&s_last, last);
+            // the first thread that passes the goal, or the last that holds anything (threads are in index order; atomics on one address of LDS took 3 us here)
+            const unsigned long long hits = __ballot(at != 0x7fffffff), lives = __ballot(last >= 0);
+            const int first = __builtin_amdgcn_readlane(at, hits ? __builtin_ctzll(hits) : 0), end = __builtin_amdgcn_readlane(last, lives ? 63 - __builtin_clzll(lives) : 0);
+            if ((tid & 63) == 0) { s_at[tid >> 6] = first; s_last[tid >> 6] = end; }
             __syncthreads();
-            pick = s_at != 0x7fffffff ? s_at : s_last;
+            at = 0x7fffffff; last = -1;
+#pragma unroll
+            for (int w = 0; w < VF_DRAW / 64; ++w) { at = min(at, s_at[w]); last = max(last, s_last[w]); }
+            pick = at != 0x7fffffff ? at : last;
             break;
         }
     }
     bad |= pick < 0;
-    for (int k = tid; k <= K; k += VF_THREADS) g.tokens[(long)b * (K + 1) + k] = bad ? -1 : k < d.accepted ? g.drafts[(long)b * K + k] : k == d.accepted ? pick : -1;
+    for (int k = tid; k <= K; k += VF_DRAW) g.tokens[(long)b * (K + 1) + k] = bad ? -1 : k < d.accepted ? g.drafts[(long)b * K + k] : k == d.accepted ? pick : -1;
     if (tid == 0) g.counts[b] = bad ? -1 : d.accepted + 1;
 }
 
@@ -417,15 +426,15 @@ int launch_verify(const VerifyArgs& g, hipStream_t s) {
         t.tokens += (int64_t)b0 * (g.max_drafts + 1);
         t.counts += b0;
         t.workspace = static_cast<char*>(g.workspace) + verify_workspace(b0, g.max_drafts, g.vocab);
-        const dim3 grid((unsigned)S, (unsigned)(t.streams * per)), block(VF_THREADS), per_stream((unsigned)t.streams);
+        const dim3 grid((unsigned)S, (unsigned)(t.streams * per)), block(VF_THREADS), per_stream((unsigned)t.streams), draw(VF_DRAW);
         if (!t.uniforms) hipLaunchKernelGGL(verify_stats_kernel<true>, grid, block, 0, s, t);
         else hipLaunchKernelGGL(verify_stats_kernel<false>, grid, block, 0, s, t);
         if (t.draft) {
-            hipLaunchKernelGGL(verify_decide_kernel, per_stream, block, 0, s, t);
+            hipLaunchKernelGGL(verify_decide_kernel, per_stream, draw, 0, s, t);
             hipLaunchKernelGGL(verify_left_kernel, dim3((unsigned)S, (unsigned)t.streams), block, 0, s, t);
-            hipLaunchKernelGGL(verify_draw_kernel<true>, per_stream, block, 0, s, t);
+            hipLaunchKernelGGL(verify_draw_kernel<true>, per_stream, draw, 0, s, t);
         } else {
-            hipLaunchKernelGGL(verify_draw_kernel<false>, per_stream, block, 0, s, t);
+            hipLaunchKernelGGL(verify_draw_kernel<false>, per_stream, draw, 0, s, t);
         }
     }
     return hipGetLastError() == hipSuccess ? ISST_OK : ISST_ERR_HIP;
