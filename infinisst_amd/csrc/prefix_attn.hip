@@ -15,6 +15,7 @@
 
 typedef __attribute__((ext_vector_type(16))) float f32x16_t;
 typedef __attribute__((ext_vector_type(4))) short s16x4_t;
+typedef __attribute__((address_space(3))) void* lds_ptr;
 
 #define PA_TILE 32               // keys of a block tile
 #define PA_RAISE 0x1p16f         // sum of a step's weights from which a column's reference exponent is raised
@@ -101,7 +102,7 @@ __device__ void add_keys(const isst_prefix_attn& a, const PrefixPlan& p, const K
 // the next tile is issued with this tile's exponentials, so that the matrix pipe and the vector ALU work at the same time (two workgroups per CU: 256 registers a lane).
 template <int D, int NW>
 __device__ __forceinline__ void block_role(const isst_prefix_attn& a, const PrefixPlan& p, char* lds, const KeySpan& w, int c0, int split, int splits, int slot) {
-    constexpr int ROWB = 2 * D, CH = D / 8, LOADS = PA_TILE * CH / (NW * 64), RSTEP = NW * 64 / CH, QS = D / 16, DT = D / 32, STAGE = 2 * PA_TILE * ROWB;
+    constexpr int ROWB = 2 * D, CH = D / 8, LOADS = PA_TILE * CH / (NW * 64), RSTEP = NW * 64 / CH, QS = D / 16, DT = D / 32, STAGE = PA_TILE * ROWB;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), c32 = lane & 31, half = lane >> 5;
     const int G = a.heads / a.kv_heads, cw = c0 + 32 * wave;
     const int total = (sees(w, (min(c0 + 32 * NW, w.ncols) - 1) / G) + PA_TILE - 1) / PA_TILE, per = (total + splits - 1) / splits, tile0 = split * per, tiles = min(per, total - tile0);
@@ -111,32 +112,29 @@ __device__ __forceinline__ void block_role(const isst_prefix_attn& a, const Pref
     const int limit = live ? sees(w, t) : w.keys, see_least = sees(w, t0), see_most = wave_live ? sees(w, (min(cw + 32, w.ncols) - 1) / G) : 0;
     const int mine = min(tiles, (see_most + PA_TILE - 1) / PA_TILE - tile0);  // tiles that this wave's columns see
 
-    const int lr = tid / CH, lc = tid % CH, kstep = (int)w.kstride * 2, vstep = (int)w.vstride * 2;
-    const unsigned koff = lr * kstep + lc * 16, voff = lr * vstep + lc * 16;
-    struct Rows { u32x4_t k[LOADS], v[LOADS]; };
-    auto fetch = [&](Rows& x, int i0) {
-        const int j0 = (tile0 + i0) * PA_TILE, rows = w.keys - j0;
-        const __amdgpu_buffer_rsrc_t kr = key_rsrc(w.k + j0 * w.kstride), vr = key_rsrc(w.v + j0 * w.vstride);
-#pragma unroll
-        for (int i = 0; i < LOADS; ++i) {
-            x.k[i] = __builtin_amdgcn_raw_buffer_load_b128(kr, lr < rows - i * RSTEP ? koff : PA_OOB, i * RSTEP * kstep, 0);
-            x.v[i] = __builtin_amdgcn_raw_buffer_load_b128(vr, lr < rows - i * RSTEP ? voff : PA_OOB, i * RSTEP * vstep, 0);
-        }
-    };
-    auto put = [&](const Rows& x, char* base) {
-#pragma unroll
-        for (int i = 0; i < LOADS; ++i) {
-            *reinterpret_cast<u32x4_t*>(base + tile_off<D>(lr + i * RSTEP, lc)) = x.k[i];
-            *reinterpret_cast<u32x4_t*>(base + PA_TILE * ROWB + tile_off<D>(lr + i * RSTEP, lc)) = x.v[i];
-        }
-    };
-    Rows staged, second;
-    if (tiles > 0) fetch(staged, 0);
-    if (tiles > 1) fetch(second, 1);
     u32x4_t qf[QS];
 #pragma unroll
     for (int s = 0; s < QS; ++s)
         qf[s] = live ? *reinterpret_cast<const u32x4_t*>(a.q + (w.first + t) * a.q_row + head * a.q_head + 16 * s + 8 * half) : (u32x4_t){0u, 0u, 0u, 0u};
+    // keys of tile i go to key stage i % 4, its values to value stage i % 4, by LDS-DMA: a wave fills 1 KB at a time in lane order, so the swizzle is in which chunk of its row a lane asks
+    // for.  Rows behind the last key repeat it.
+    const int lr = tid / CH, lc = tile_off<D>(lr, tid % CH) % ROWB;
+    const long krows = RSTEP * 2 * w.kstride, vrows = RSTEP * 2 * w.vstride;  // bytes between the rows of two loads
+    unsigned koff = lr * (int)(2 * w.kstride) + lc, voff = lr * (int)(2 * w.vstride) + lc;
+    char *const kring = lds, *const vring = lds + 4 * STAGE;
+    auto stage = [&](int i) { return (i & 3) * STAGE; };
+    auto fetch = [&](const bf16_t* rows0, long stride, int i, char* stage) {
+        const int left = w.keys - (tile0 + i) * PA_TILE;
+        if (i >= tiles) return;
+        const char* src = reinterpret_cast<const char*>(rows0 + (tile0 + i) * PA_TILE * stride);
+#pragma unroll
+        for (int k = 0; k < LOADS; ++k)
+            __builtin_amdgcn_global_load_lds((const void*)(src + (unsigned)(min(lr + k * RSTEP, left - 1) * (int)(2 * stride) + lc)), (lds_ptr)(stage + (k * NW + wave) * 1024), 16, 0, 0);
+    };
+    fetch(w.k, w.kstride, 0, kring);
+    fetch(w.k, w.kstride, 1, kring + STAGE);
+    fetch(w.k, w.kstride, 2, kring + 2 * STAGE);
+    fetch(w.v, w.vstride, 0, vring);
     f32x16_t o[DT];
 #pragma unroll
     for (int d = 0; d < DT; ++d)
@@ -146,34 +144,32 @@ __device__ __forceinline__ void block_role(const isst_prefix_attn& a, const Pref
     unsigned ill_tiles = 0;
     const float c2 = a.scale * 1.44269504088896340736f;  // exp(scale s - ..) = exp2(c2 s - ..)
 
-    char *cur = lds, *next = lds + STAGE, *spare = lds + 2 * STAGE;
-    if (tiles > 0) put(staged, cur);
-    if (tiles > 2) fetch(staged, 2);
-    if (tiles > 1) put(second, next);
-    __syncthreads();
-#pragma unroll
-    for (int s = 0; s < QS; ++s) asm volatile("" : "+v"(qf[s]));  // (the queries have landed: a wait for them inside the loop would wait for the newest tile as well)
-    auto scores = [&](const char* kt) {
+    // everything asked for has landed, for every wave, and every wave is done with what it read
+    auto turn = [&]() {
+        asm volatile("" ::: "memory");
+        __builtin_amdgcn_s_waitcnt(0x70);  // vmcnt(0) lgkmcnt(0)
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+    };
+    turn();
+    // LDS offsets of a lane inside its stage; other product steps and columns are an XOR away (the swizzle is one), other rows a constant
+    const int klane = tile_off<D>(c32, half), vlane = tile_off<D>(4 * half + ((lane >> 2) & 3), 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1)) + 8 * (lane & 1);
+    auto key_frag = [&](const char* kst, int s) { return __builtin_bit_cast(bf16x8_t, *reinterpret_cast<const u32x4_t*>(kst + (klane ^ 32 * s))); };
+    // 16 keys a product: slots j < 4 of half h = keys 16 k + 4 h + j, j >= 4 = keys 16 k + 8 + 4 h + (j - 4)
+    auto value_frag = [&](const char* vst, int k, int d) {
+        const u32x2_t v1 = read_tr(vst + (vlane ^ 64 * d) + 16 * k * ROWB), v2 = read_tr(vst + (vlane ^ (64 * d + 32)) + (16 * k + 8) * ROWB);
+        return __builtin_bit_cast(bf16x8_t, (u32x4_t){v1.x, v1.y, v2.x, v2.y});
+    };
+    auto scores = [&](const char* kst) {
         f32x16_t sc;
 #pragma unroll
         for (int r = 0; r < 16; ++r) sc[r] = 0.f;
 #pragma unroll
-        for (int s = 0; s < QS; ++s) {
-            const u32x4_t kf = *reinterpret_cast<const u32x4_t*>(kt + tile_off<D>(c32, 2 * s + half));
-            sc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8_t, kf), __builtin_bit_cast(bf16x8_t, qf[s]), sc, 0, 0, 0);
-        }
+        for (int s = 0; s < QS; ++s) sc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(key_frag(kst, s), __builtin_bit_cast(bf16x8_t, qf[s]), sc, 0, 0, 0);
         return sc;
     };
-    f32x16_t sc = scores(cur);  // (no tile: of whatever the stage holds, unused -- as behind the last tile below)
-    auto stage = [&](int i) {
-        if (i + 2 < tiles) put(staged, spare);
-        if (i + 3 < tiles) fetch(staged, i + 3);
-    };
-    auto turn = [&]() {
-        __syncthreads();
-        char* done = cur;
-        cur = next; next = spare; spare = done;
-    };
+    f32x16_t sc = scores(kring);  // (no tile: of whatever the stage holds, unused -- as behind the last tile below)
+    turn();                       // (keys 4 take the place of keys 0)
     // m becomes the maximum of what it covers and of these scores
     auto raise = [&]() {
         float mx = sc[0];
@@ -203,62 +199,131 @@ __device__ __forceinline__ void block_role(const isst_prefix_attn& a, const Pref
             }
         return sum;
     };
-    // One tile: its scores are in sc, those of the next are computed on the way.  EDGE: some column does not see some key of it.
+    // Step i: the scores of tile i are in sc and become weights; on the way the values of tile i - 1, whose weights are in pf, are added and the scores of tile i + 1 are computed.
     // A column's reference m is the maximum of its first tile (and of its edge tiles): weights are exponentials against it, bf16 and fp32 hold them to 2^127, and no bit is lost by their
     // size.  So other maxima are not looked for -- that and the running sum were 100 of the 169 vector instructions of a tile -- and only weights that pass PA_RAISE (or NaN) move m,
     // before anything of the tile was used.
-    auto step = [&](int i, auto edge) {
-        constexpr bool EDGE = decltype(edge)::value;
-        stage(i);
-        const char* vt = cur + PA_TILE * ROWB;
-        const int j0 = (tile0 + i) * PA_TILE;
-        bool ill = false;  // inf or NaN among the values
-        if constexpr (EDGE) {
-            const int lim = limit - j0 - 4 * half;
-#pragma unroll
-            for (int r = 0; r < 16; ++r)
-                if ((r & 3) + 8 * (r >> 2) >= lim) sc[r] = -INFINITY;
-            raise();
+    u32x4_t pf[2];
+    enum { NONE, WHOLE, EDGE } before = NONE;  // what tile i - 1 was: EDGE, some column did not see some key of it
+    auto ref = [&]() { return m == -INFINITY ? 0.f : -m; };
+    auto add_values = [&](int i) {  // of tile i
+        if (before == EDGE) {
+            bool ill = false;  // inf or NaN among the values: they are added behind the loop
 #pragma unroll 1
             for (int k = 0; k < PA_TILE * ROWB / 1024; ++k) {
-                const u32x4_t v = *reinterpret_cast<const u32x4_t*>(vt + 1024 * k + 16 * lane);
+                const u32x4_t v = *reinterpret_cast<const u32x4_t*>(vring + (i & 3) * STAGE + 1024 * k + 16 * lane);
 #pragma unroll
                 for (int e = 0; e < 4; ++e) ill |= (v[e] & 0x7f80u) == 0x7f80u || (v[e] & 0x7f800000u) == 0x7f800000u;
             }
-            ill = __any(ill);
-        }
-        u32x4_t pf[2];
-        auto at = [&]() { return m == -INFINITY ? 0.f : -m; };
-        float sum = weights(pf, EDGE ? at() : -m);  // (no reference yet, all scores so far -inf: weights of inf, or NaN, which set one)
-        if constexpr (!EDGE)
-            if (__any(!(sum <= PA_RAISE))) {
-                raise();
-                sum = weights(pf, at());
+            if (__any(ill)) {
+                ill_tiles |= 1u << min((tile0 + i) - see_least / PA_TILE, 31);
+                return;
             }
-        l += sum;
-        const f32x16_t sn = scores(next);
-        if (!EDGE || !ill) {
-#pragma unroll
-            for (int k = 0; k < 2; ++k)  // 16 keys: slots j < 4 of half h = keys 16 k + 4 h + j, j >= 4 = keys 16 k + 8 + 4 h + (j - 4)
-#pragma unroll
-                for (int d = 0; d < DT; ++d) {
-                    const int ch = 4 * d + 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1), r = 16 * k + 4 * half + ((lane >> 2) & 3);
-                    const u32x2_t v1 = read_tr(vt + tile_off<D>(r, ch) + 8 * (lane & 1)), v2 = read_tr(vt + tile_off<D>(r + 8, ch) + 8 * (lane & 1));
-                    const u32x4_t vf = {v1.x, v1.y, v2.x, v2.y};
-                    o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8_t, vf), __builtin_bit_cast(bf16x8_t, pf[k]), o[d], 0, 0, 0);
-                }
-        } else {  // the tile's values are added behind the loop
-            ill_tiles |= 1u << min((tile0 + i) - see_least / PA_TILE, 31);
         }
+#pragma unroll
+        for (int k = 0; k < 2; ++k)
+#pragma unroll
+            for (int d = 0; d < DT; ++d) o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(value_frag(vring + (i & 3) * STAGE, k, d), __builtin_bit_cast(bf16x8_t, pf[k]), o[d], 0, 0, 0);
+    };
+    // the first tile and those at the edge: one thing after the other
+    auto slow_step = [&](int i, bool edge) {
+        if (before != NONE) add_values(i - 1);
+        if (edge) {
+            const int lim = limit - (tile0 + i) * PA_TILE - 4 * half;
+#pragma unroll
+            for (int r = 0; r < 16; ++r)
+                if ((r & 3) + 8 * (r >> 2) >= lim) sc[r] = -INFINITY;
+        }
+        raise();
+        l += weights(pf, ref());
+        before = edge ? EDGE : WHOLE;
+        sc = scores(kring + stage(i + 1));
+    };
+    // the others: matrix and vector instructions in turn, since the two waves of a SIMD do not find enough of the other's kind by themselves
+    auto step = [&](const char* __restrict__ kst, const char* __restrict__ vst) {
+        bf16x8_t kf[QS], vf[2][DT];
+#pragma unroll
+        for (int s = 0; s < QS / 2; ++s) kf[s] = key_frag(kst, s);
+#pragma unroll
+        for (int d = 0; d < DT; ++d) vf[0][d] = value_frag(vst, 0, d);
+        __builtin_amdgcn_sched_barrier(0);
+        const bf16x2_t one = {(__bf16)1.f, (__bf16)1.f};
+        f32x16_t sn;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) sn[r] = 0.f;
+        u32x4_t pn[2];
+        float sum = 0.f;
+        constexpr int EVERY = 8 / QS;
+#pragma unroll
+        for (int c = 0; c < 8; ++c) {
+            const int q = c / EVERY;
+            if (c % EVERY == 0) {
+                sn = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf[q], __builtin_bit_cast(bf16x8_t, qf[q]), sn, 0, 0, 0);
+                if (q < QS / 2) kf[q + QS / 2] = key_frag(kst, q + QS / 2);
+            }
+            const float e0 = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[2 * c], c2, -m)), e1 = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[2 * c + 1], c2, -m));
+            if (c % EVERY == 0) {
+                o[q % DT] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf[q / DT][q % DT], __builtin_bit_cast(bf16x8_t, pf[q / DT]), o[q % DT], 0, 0, 0);
+                if (q < DT) vf[1][q] = value_frag(vst, 1, q);
+            }
+            const uint32_t pair = pack_bf(e0, e1);
+            pn[c / 4][c % 4] = pair;
+            sum = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2_t, pair), one, sum, false);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        if (__any(!(sum <= PA_RAISE))) {  // (no reference yet, all scores so far -inf: weights of inf or NaN, which set one)
+            raise();
+            sum = weights(pn, ref());
+        }
+        l += sum;
+        pf[0] = pn[0]; pf[1] = pn[1];
         sc = sn;
-        turn();
     };
     const int whole = min(mine, see_least / PA_TILE - tile0);  // tiles that every column of the wave sees whole
-    if (whole > 0) raise();
+    // Two tiles between barriers: keys i + 1, i + 2 and values i - 1, i are read while keys i + 3, i + 4 and values i + 1, i + 2 arrive
+    const char *ksrc = reinterpret_cast<const char*>(w.k + (tile0 + 3) * PA_TILE * w.kstride), *vsrc = reinterpret_cast<const char*>(w.v + (tile0 + 1) * PA_TILE * w.vstride);
+    auto ask = [&](int i, char* __restrict__ knew0, char* __restrict__ knew1, char* __restrict__ vnew0, char* __restrict__ vnew1) {
+        if (i + 5 < tiles) {
+            asm volatile("" : "+v"(koff), "+v"(voff));  // (32-bit offsets to the scalar bases, not 64-bit addresses kept in registers)
+#pragma unroll
+            for (int k = 0; k < LOADS; ++k) {
+                __builtin_amdgcn_global_load_lds((const void*)(ksrc + k * krows + koff), (lds_ptr)(knew0 + (k * NW + wave) * 1024), 16, 0, 0);
+                __builtin_amdgcn_global_load_lds((const void*)(ksrc + (k + LOADS) * krows + koff), (lds_ptr)(knew1 + (k * NW + wave) * 1024), 16, 0, 0);
+                __builtin_amdgcn_global_load_lds((const void*)(vsrc + k * vrows + voff), (lds_ptr)(vnew0 + (k * NW + wave) * 1024), 16, 0, 0);
+                __builtin_amdgcn_global_load_lds((const void*)(vsrc + (k + LOADS) * vrows + voff), (lds_ptr)(vnew1 + (k * NW + wave) * 1024), 16, 0, 0);
+            }
+            ksrc += 2 * LOADS * krows;
+            vsrc += 2 * LOADS * vrows;
+        } else {
+            fetch(w.k, w.kstride, i + 3, knew0);
+            fetch(w.k, w.kstride, i + 4, knew1);
+            fetch(w.v, w.vstride, i + 1, vnew0);
+            fetch(w.v, w.vstride, i + 2, vnew1);
+        }
+    };
+    auto two_steps = [&](int i, char* __restrict__ knew0, char* __restrict__ knew1, char* __restrict__ vnew0, char* __restrict__ vnew1, const char* __restrict__ kst0,
+                         const char* __restrict__ kst1, const char* __restrict__ vst0, const char* __restrict__ vst1) {
+        ask(i, knew0, knew1, vnew0, vnew1);
+        step(kst0, vst0);
+        step(kst1, vst1);
+        turn();
+    };
     int i = 0;
-    for (; i < whole; ++i) step(i, std::integral_constant<bool, false>{});
-    for (; i < mine; ++i) step(i, std::integral_constant<bool, true>{});
-    for (; i < tiles; ++i) { stage(i); turn(); }
+    while (i < ((tiles + 1) & ~1)) {
+        if (!(i & 1)) ask(i, kring + stage(i + 3), kring + stage(i), vring + stage(i + 1), vring + stage(i + 2));
+        if (i < mine) slow_step(i, i >= whole);
+        else if (before != NONE) {
+            add_values(i - 1);
+            before = NONE;
+        }
+        if (i & 1) turn();
+        ++i;
+        if (!(i & 1))
+            for (; i + 1 < whole; i += 2)
+                two_steps(i, kring + stage(i + 3), kring + stage(i), vring + stage(i + 1), vring + stage(i + 2), kring + stage(i + 1), kring + stage(i + 2), vring + stage(i + 3), vring + stage(i));
+    }
+    if (before != NONE) add_values(mine - 1);
+    __syncthreads();  // (the last values are read behind the last turn)
     // ---- (m, l) and the accumulators; these turn through the wave's part of LDS so that whole rows of D floats are stored ----
     int jl = lane;
     asm volatile("" : "+v"(jl));
@@ -320,7 +385,8 @@ __device__ __forceinline__ void span_role(const isst_prefix_attn& a, const Prefi
 #pragma unroll
         for (int i = 0; i < VL; ++i) vr[i] = __builtin_amdgcn_raw_buffer_load_b128(r, lane / CH < see_most - j0 - i * VR ? voff : PA_OOB, i * VR * vstep, 0);
     };
-    __shared__ unsigned ill_steps;
+    float2* wml = reinterpret_cast<float2*>(lds + NW * 32 * D * 4);  // [NW][16 NQ], behind the value tiles / turned accumulators
+    unsigned& ill_steps = *reinterpret_cast<unsigned*>(wml + NW * 16 * NQ);
     if (tid == 0) ill_steps = 0;
     __syncthreads();
     const int step = 32 * NW * splits;
@@ -451,12 +517,11 @@ __device__ __forceinline__ void span_role(const isst_prefix_attn& a, const Prefi
     int jt = tid;
     asm volatile("" : "+v"(jt));  // (keeps this part's addresses out of the registers of the loop above)
     const int jc = jt & 15, jq = (jt & 63) >> 4;
-    __shared__ float2 wml[NW][16 * NQ];
 #pragma unroll
     for (int n = 0; n < NQ; ++n) {
         l[n] += __shfl_xor(l[n], 16, WAVE);
         l[n] += __shfl_xor(l[n], 32, WAVE);
-        if (jq == 0) wml[wave][16 * n + jc] = make_float2(m[n], l[n]);
+        if (jq == 0) wml[wave * 16 * NQ + 16 * n + jc] = make_float2(m[n], l[n]);
     }
     __syncthreads();  // (also: every wave is done with its value tile, which the accumulators overlay)
     float* red = reinterpret_cast<float*>(lds);  // [NW][16 columns][D]
@@ -464,10 +529,10 @@ __device__ __forceinline__ void span_role(const isst_prefix_attn& a, const Prefi
     for (int n = 0; n < NQ; ++n) {
         float M = -INFINITY, L = 0.f;
 #pragma unroll
-        for (int w = 0; w < NW; ++w) M = fmaxf(M, wml[w][16 * n + jc].x);
+        for (int w = 0; w < NW; ++w) M = fmaxf(M, wml[w * 16 * NQ + 16 * n + jc].x);
 #pragma unroll
         for (int w = 0; w < NW; ++w) {
-            const float2 x = wml[w][16 * n + jc];
+            const float2 x = wml[w * 16 * NQ + 16 * n + jc];
             L += x.x == -INFINITY ? x.y : x.y * __builtin_amdgcn_exp2f(x.x - M);
         }
         const float keep = m[n] == -INFINITY ? (l[n] == 0.f ? 0.f : 1.f) : __builtin_amdgcn_exp2f(m[n] - M);
@@ -499,7 +564,7 @@ __device__ __forceinline__ void span_role(const isst_prefix_attn& a, const Prefi
 
 template <int D, int NW, int NQ>
 __global__ __launch_bounds__(NW * 64, 2) void prefix_attn_partial_kernel(isst_prefix_attn a, PrefixPlan p) {
-    constexpr int BLOCK_LDS = 3 * 2 * PA_TILE * 2 * D, SPAN_LDS = NW * 32 * D * 4;  // (ring of three stages; the turned accumulators of a block, the value tiles and the join of a span)
+    constexpr int BLOCK_LDS = 4 * 2 * PA_TILE * 2 * D, SPAN_LDS = NW * 32 * D * 4 + NW * 16 * NQ * 8 + 16;  // (ring of three stages; the turned accumulators of a block, the value tiles and the join of a span)
     __shared__ __attribute__((aligned(16))) char lds[BLOCK_LDS > SPAN_LDS ? BLOCK_LDS : SPAN_LDS];
     // workgroup i runs on XCD i % 8 (each with an L2 of its own): the column tiles that read the same keys are neighbours on one XCD
     const bool prefix = (int)blockIdx.x < p.prefix_units;
