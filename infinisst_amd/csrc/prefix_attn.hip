@@ -367,10 +367,21 @@ __device__ __forceinline__ void span_role(const isst_prefix_attn& a, const Prefi
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), fr = lane & 15, fq = lane >> 4;
     const int G = a.heads / a.kv_heads, t0 = c0 / G, x0 = c0 % G;
     const int see_least = sees(w, t0), see_most = sees(w, (min(c0 + 16 * NQ, w.ncols) - 1) / G);
-    char* vl = lds + wave * (32 * ROWB);
-    u32x4_t kf[2][QS], vr[VL];
+    char* vl = lds + wave * (64 * ROWB);  // two tiles of 32 values, this wave's alone
+    u32x4_t kf[2][QS];
     const int kstep = (int)w.kstride * 2, vstep = (int)w.vstride * 2;
-    const unsigned koff = fr * kstep + 16 * fq, voff = lane / CH * vstep + 16 * (lane % CH);
+    const unsigned koff = fr * kstep + 16 * fq;
+    // values come by LDS-DMA, in front of the keys of the same step: the wait for these is the wait for them
+    const int lr = lane / CH;
+    auto fetch_v = [&](int j0, char* dst) {
+        const char* src = reinterpret_cast<const char*>(w.v + j0 * w.vstride);
+        const int last = see_most - 1 - j0;
+#pragma unroll
+        for (int i = 0; i < VL; ++i) {
+            const int row = lr + i * VR, lc = tile_off<D>(row, lane % CH) % ROWB;
+            __builtin_amdgcn_global_load_lds((const void*)(src + (unsigned)(min(row, last) * vstep + lc)), (lds_ptr)(dst + 1024 * i), 16, 0, 0);
+        }
+    };
     auto fetch_k = [&](int j0) {
         const __amdgpu_buffer_rsrc_t r = key_rsrc(w.k + j0 * w.kstride);
 #pragma unroll
@@ -380,18 +391,13 @@ __device__ __forceinline__ void span_role(const isst_prefix_attn& a, const Prefi
             for (int s = 0; s < QS; ++s) kf[t][s] = __builtin_amdgcn_raw_buffer_load_b128(r, off, 16 * t * kstep + 64 * s, 0);
         }
     };
-    auto fetch_v = [&](int j0) {
-        const __amdgpu_buffer_rsrc_t r = key_rsrc(w.v + j0 * w.vstride);
-#pragma unroll
-        for (int i = 0; i < VL; ++i) vr[i] = __builtin_amdgcn_raw_buffer_load_b128(r, lane / CH < see_most - j0 - i * VR ? voff : PA_OOB, i * VR * vstep, 0);
-    };
     float2* wml = reinterpret_cast<float2*>(lds + NW * 32 * D * 4);  // [NW][16 NQ], behind the value tiles / turned accumulators
     unsigned& ill_steps = *reinterpret_cast<unsigned*>(wml + NW * 16 * NQ);
     if (tid == 0) ill_steps = 0;
     __syncthreads();
     const int step = 32 * NW * splits;
     int j0 = 32 * (split * NW + wave);
-    if (j0 < see_most) { fetch_v(j0); fetch_k(j0); }
+    if (j0 < see_most) { fetch_v(j0, vl); fetch_k(j0); }
 
     int limit[NQ];
     u32x4_t qf[NQ][QS];
@@ -413,11 +419,10 @@ __device__ __forceinline__ void span_role(const isst_prefix_attn& a, const Prefi
     }
     const float c2 = a.scale * 1.44269504088896340736f;
     bool first_step = true;
+    int turn = 0;
     for (; j0 < see_most; j0 += step) {
-#pragma unroll
-        for (int i = 0; i < VL; ++i) *reinterpret_cast<u32x4_t*>(vl + tile_off<D>(i * VR + lane / CH, lane % CH)) = vr[i];
         const bool more = j0 + step < see_most;
-        if (more) fetch_v(j0 + step);
+        char* const vt = vl + (turn & 1) * (32 * ROWB);
         __builtin_amdgcn_sched_barrier(0);
         f32x4_t sc[NQ][2];
 #pragma unroll
@@ -430,7 +435,19 @@ __device__ __forceinline__ void span_role(const isst_prefix_attn& a, const Prefi
                     sc[n][t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, kf[t][s]), __builtin_bit_cast(bf16x8_t, qf[n][s]), sc[n][t], 0, 0, 0);
             }
         __builtin_amdgcn_sched_barrier(0);
-        if (more) fetch_k(j0 + step);
+        const int vrow = 4 * fq + ((lane >> 2) & 3), vch = (lane & 3) >> 1, vb8 = 8 * (lane & 1);
+        bf16x8_t vf[NT];
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+            const u32x2_t v1 = read_tr(vt + tile_off<D>(vrow, 2 * t + vch) + vb8), v2 = read_tr(vt + tile_off<D>(16 + vrow, 2 * t + vch) + vb8);
+            vf[t] = __builtin_bit_cast(bf16x8_t, (u32x4_t){v1.x, v1.y, v2.x, v2.y});
+        }
+        __builtin_amdgcn_sched_barrier(0);
+        if (more) {
+            fetch_v(j0 + step, vl + (~turn & 1) * (32 * ROWB));
+            fetch_k(j0 + step);
+        }
+        ++turn;
         __builtin_amdgcn_sched_barrier(0);
         const bool edge = j0 + 32 > see_least;  // some column does not see some key of this step
         auto raise = [&]() {  // m becomes the maximum of what it covers and of these scores
@@ -493,7 +510,7 @@ __device__ __forceinline__ void span_role(const isst_prefix_attn& a, const Prefi
             bool ill = false;  // inf or NaN among the values of a step that not every column sees whole
 #pragma unroll 1
             for (int i = 0; i < VL; ++i) {
-                const u32x4_t v = *reinterpret_cast<const u32x4_t*>(vl + 1024 * i + 16 * lane);
+                const u32x4_t v = *reinterpret_cast<const u32x4_t*>(vt + 1024 * i + 16 * lane);
 #pragma unroll
                 for (int w = 0; w < 4; ++w) ill |= (v[w] & 0x7f80u) == 0x7f80u || (v[w] & 0x7f800000u) == 0x7f800000u;
             }
@@ -502,16 +519,10 @@ __device__ __forceinline__ void span_role(const isst_prefix_attn& a, const Prefi
                 continue;
             }
         }
-        const int vrow = 4 * fq + ((lane >> 2) & 3), vch = (lane & 3) >> 1, vb8 = 8 * (lane & 1);
 #pragma unroll
-        for (int t = 0; t < NT; ++t) {
-            const u32x2_t v1 = read_tr(vl + tile_off<D>(vrow, 2 * t + vch) + vb8), v2 = read_tr(vl + tile_off<D>(16 + vrow, 2 * t + vch) + vb8);
-            const u32x4_t vf = {v1.x, v1.y, v2.x, v2.y};
-            if (t % 4 == 3) __builtin_amdgcn_sched_barrier(0);  // (four fragments ahead at most: more of them spill)
+        for (int t = 0; t < NT; ++t)
 #pragma unroll
-            for (int n = 0; n < NQ; ++n)
-                o[n][t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, vf), __builtin_bit_cast(bf16x8_t, pf[n]), o[n][t], 0, 0, 0);
-        }
+            for (int n = 0; n < NQ; ++n) o[n][t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf[t], __builtin_bit_cast(bf16x8_t, pf[n]), o[n][t], 0, 0, 0);
     }
     // ---- join the waves: statistics first, then the weighted accumulators of 16 columns at a time ----
     int jt = tid;
@@ -646,7 +657,7 @@ __global__ __launch_bounds__(256) void prefix_attn_join_kernel(isst_prefix_attn 
 #define PA_NW 4
 #endif
 #ifndef PA_TAU
-#define PA_TAU 1.25
+#define PA_TAU 1.0
 #endif
 #ifndef PA_FIX
 #define PA_FIX 5.0
