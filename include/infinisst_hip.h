@@ -292,7 +292,8 @@ int isst_op_gemm_attn_merge(const float* partial, int n_splits, const uint16_t* 
 /* Attention of `rows` query rows of `seqs` sequences that share a prefix of prefix_len keys in front of keys of their own (the batched form of patch_llm.py:320-329's
  * softmax(q k^T) v, keys already rotated).  Sequence b owns rows row_starts[b] .. row_starts[b + 1] - 1 (NULL: rows / seqs each) = its newest positions: row t of n
  * sees every prefix key and the own keys 0 .. tail_lens[b] - n + t.  A row that sees no key gives zeros; rows outside every sequence are left as they were.
- * Strides in elements (multiples of 8, a key's 0 .. 2^24), every row of head_dim elements contiguous and 16-byte aligned.  tail_lens is read as clamped to 0 .. tail_cap, row_starts (non-decreasing)
+ * Strides in elements (multiples of 8, a key's 0 .. 2^24), every row of head_dim elements contiguous and 16-byte aligned; rows * heads <= 2^26, heads <= 2^15,
+ * seqs * kv_heads <= 2^22.  tail_lens is read as clamped to 0 .. tail_cap, row_starts (non-decreasing)
  * to 0 .. rows: nothing outside the arrays is touched whatever they hold. */
 typedef struct isst_prefix_attn {
     const uint16_t* q;              /* [rows][heads][head_dim] */
@@ -312,7 +313,8 @@ typedef struct isst_prefix_attn {
 int64_t isst_op_prefix_attention_workspace(const isst_prefix_attn* a); /* bytes (16-byte aligned memory), < 0: bad arguments */
 int isst_op_prefix_attention(const isst_prefix_attn* a, void* workspace, int64_t workspace_bytes, void* hip_stream);
 /* out[m] = bf16(A[m] W^T + scales[a] * (A[m] down[a]^T) up[a]^T), a = row_adapter[m]; a row whose a is outside 0 .. n_adapters - 1 has no adapter.  packed:
- * isst_op_pack_weight of W [N][K]; down [n_adapters][rank][K], up [n_adapters][N][rank] bf16 contiguous; rank a multiple of 8 up to 128; K % 32 == 0.
+ * isst_op_pack_weight of W [N][K]; down [n_adapters][rank][K], up [n_adapters][N][rank] bf16 contiguous; rank a multiple of 8 up to 128; K % 32 == 0; M * K and M * lda
+ * < 2^29, M * N < 2^30.
  * Sums stay in fp32, one rounding at the end.  F.linear next to per-request adapters; the reference has one set of weights per language pair instead. */
 int64_t isst_op_gemm_lora_workspace(int M, int N, int K, int rank, int n_adapters);
 int isst_op_gemm_lora(const uint16_t* A, int64_t lda, const uint16_t* packed, const uint16_t* down, const uint16_t* up, const float* scales,

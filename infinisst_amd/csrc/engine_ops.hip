@@ -259,7 +259,7 @@ static bool prefix_attention_ok(const isst_prefix_attn* a) {
     if (!a || a->rows < 0 || a->seqs < 0 || a->max_rows < 0 || a->heads < 1 || a->kv_heads < 1 || a->heads % a->kv_heads || (a->head_dim != 64 && a->head_dim != 128) ||
         a->prefix_len < 0 || a->tail_cap < 0 || !(a->scale > 0.f) || !(a->scale < INFINITY))
         return false;
-    if (a->heads > (1 << 15) || (int64_t)a->rows * a->heads > (1 << 30) || (int64_t)a->seqs * a->kv_heads > (1 << 24) || (a->rows > 0 && a->seqs < 1)) return false;
+    if (a->heads > (1 << 15) || (int64_t)a->rows * a->heads > (1 << 26) || (int64_t)a->seqs * a->kv_heads > (1 << 22) || (a->rows > 0 && a->seqs < 1)) return false;
     if (!a->row_starts && a->seqs > 0 && a->rows % a->seqs) return false;
     if (a->rows == 0) return true;
     if (!a->q || !a->out || !a->tail_lens || !aligned16(a->q) || !aligned16(a->out)) return false;
@@ -273,7 +273,7 @@ static bool prefix_attention_ok(const isst_prefix_attn* a) {
         strides |= a->kt_seq | a->kt_head | a->kt_key | a->vt_seq | a->vt_head | a->vt_key;
     }
     if (strides & 7) return false;
-    for (const int64_t key : {a->kp_key, a->vp_key, a->kt_key, a->vt_key})  // (32-bit offsets inside a tile of 64 keys)
+    for (const int64_t key : {a->kp_key, a->vp_key, a->kt_key, a->vt_key})  // (32-bit offsets inside a tile of 32 keys)
         if (key < 0 || key > (1 << 24)) return false;
     // two outputs never share memory
     return (a->heads == 1 || a->out_head >= a->head_dim) && (a->rows == 1 || a->out_row >= (a->heads - 1) * a->out_head + a->head_dim);
@@ -294,7 +294,8 @@ static GemmArgs lora_base_args(const uint16_t* A, int64_t lda, const uint16_t* p
     g.A = A; g.lda = lda; g.Wp = packed; g.out = base; g.N = round_up(N, 16); g.ldo = g.N; g.out_batch = (long)M * g.N;
     g.M = M; g.K = K; g.batch = 1; g.n_valid = N;
     g.epi = EPI_PARTIAL;
-    // as many K slices as give every compute unit a workgroup of that kernel, in one round
+    // as many K slices as give every compute unit a workgroup of that kernel, in one round (the base in us, slices 1 / 2 / 4: 64 rows of 4096 x 6144 23 / 18 / 23, 1408 rows of 4096 x 4096
+    // 78 / 52 / 61; slices 2 / 4 / 8: 320 rows of 14336 x 4096 120 / 72 / 50)
     g.ksplit = 1;
     if (M > 64 && !gemm_dense_would_run(M, g.N, K)) g.ksplit = pick_ksplit(K, g.N, M, 1L << 28);
     else if (M > 12) {

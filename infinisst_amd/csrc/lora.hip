@@ -4,6 +4,8 @@
 // Both kernels take tiles of 16 rows and walk the DISTINCT adapters of a tile: one matrix product per adapter for all 16 rows, of which every row keeps the one of its own adapter -- a
 // selection, so that another adapter's inf or NaN cannot reach it.  No sorting and no plan: neighbouring rows of a stream share an adapter (one or two products a tile), and a decode
 // step with an adapter per row reads each adapter once, as it has to.  Bound by the adapters' bytes and, below them, by latency.
+// Measured next to their base product (us, down + base + up; K x N, rank, rows): 4096 x 6144, 16, 1 row 3.9 + 8.9 + 3.9; 64 rows with 64 adapters 5.3 + 18 + 7.0; 14336 x 4096, 64, 320 rows
+// 16.5 + 49 + 17; 4096 x 4096, 32, 1408 rows 10 + 51 + 19.
 #include "common.h"
 #include "kernels.h"
 
@@ -11,9 +13,7 @@
 #define LORA_DOWN_WAVES 4
 #define LORA_STEPS 4                                     // 32-deep product steps of a wave
 #define LORA_DOWN_K (LORA_DOWN_WAVES * LORA_STEPS * 32)  // K slice of a workgroup
-#ifndef LORA_WIDE
-#define LORA_WIDE 256  // workgroups from which a row tile takes 256 columns
-#endif
+#define LORA_WIDE 256  // workgroups of 256 columns a row tile from which these are taken instead of 64
 
 // the tile's adapters: id of row lane & 15 in every lane (-1: none), and which rows are the first of their adapter
 __device__ __forceinline__ int tile_ids(const LoraArgs& g, int m0, unsigned& leaders) {
@@ -36,7 +36,8 @@ __device__ __forceinline__ int xcd_unit(int i, int total) {
     return (i >> 3) < per && u < total ? u : -1;
 }
 
-// t[slice][m][r] = the K slice's part of down[a][r] . x[m].  Units: row tile fastest, then z of Z, then K slice; adapter j of a tile belongs to z = j mod Z
+// t[slice][m][r] = the K slice's part of down[a][r] . x[m].  Slices of 512 = four waves x four product steps (256 or 1024 a workgroup: 1408 rows 10 -> 11 or 12.5 us, 320 rows 16.5 -> 15 or 20,
+// and the up kernel has twice or half the slices to add: 17 -> 20 or 17; 32-row tiles: the same).  Units: row tile fastest, then z of Z, then K slice; adapter j of a tile belongs to z = j mod Z
 template <int RT>  // rank tiles of 16
 __global__ __launch_bounds__(LORA_DOWN_WAVES * 64) void lora_down_kernel(LoraArgs g, int tiles, int Z, int units) {
     __shared__ float red[LORA_DOWN_WAVES][LORA_ROWS][RT * 16];
@@ -99,7 +100,8 @@ __global__ __launch_bounds__(LORA_DOWN_WAVES * 64) void lora_down_kernel(LoraArg
 }
 
 // Units: row tile fastest, then column tile of 64 CG.  t enters the product as a pair of bf16 numbers (hi, lo: 2^-16 relative) side by side along the product's depth, both against the same entries
-// of up.  CG = 1: the waves take an adapter each (few workgroups: decode steps); CG = 4: a column group each (t is summed once for 256 columns)
+// of up.  CG = 1: the waves take an adapter each (few workgroups: decode steps; 64 rows with 64 adapters 6.9 us, with CG = 4 13.5); CG = 4: a column group each
+// (t is summed once for 256 columns: 1408 rows 19 us, with CG = 1 26).  Bound by the base's fp32 slices: 46 MB at 1408 rows, 42 MB at 320
 template <int RT, int CG>
 __global__ __launch_bounds__(256) void lora_up_kernel(LoraArgs g, int tiles, int units) {
     constexpr int LD = RT * 16 + 8;  // (row padding: the rows of a fragment start in different banks)

@@ -1,12 +1,17 @@
 // Attention of a batch whose sequences share one long prefix in front of keys of their own (gfx950).
 //
 // Row t of the n rows of sequence b sees the P prefix keys and its own keys j < len_b - n + t + 1:
-//     o = sum_j exp(scale q.k_j - m) v_j / sum_j exp(scale q.k_j - m)   over both sets, m = the running maximum.
+//     o = sum_j exp(scale q.k_j - m) v_j / sum_j exp(scale q.k_j - m)   over both sets, for any m that keeps the exponentials in range (m: the column's reference).
 // One launch computes partial (O, m, l) triples, a second one joins them.  A workgroup of the first launch takes one of two roles:
-//   block: 32 NW columns ((row, head) pairs of one key head, over ALL sequences) against a span of the prefix.  Every K / V tile of 64 keys goes through LDS once for all columns.
-//   span:  16 NQ columns of ONE sequence against its own keys (or of the whole batch against the prefix where it has no more columns than that); the waves split the keys.
+//   block: 32 NW columns ((row, head) pairs of one key head, over ALL sequences) against a span of the prefix, or the columns of one sequence against its own keys.  Every tile of 32 keys
+//          goes through LDS once for all columns.  Bound by the matrix instructions and what goes with them.
+//   span:  16 NQ columns of ONE sequence against its own keys (or of the whole batch against the prefix where it has no more columns than that); the waves split the keys.  Bound by the read.
 // Scores are computed transposed, S^T = K Q^T, so that a lane holds one column: statistics and rescaling are per lane, and the exponentials are already in the layout the value product
 // O^T = V^T P^T wants its B operand in (the order of the keys inside a 16- or 32-key step is free as long as V^T is read in the same order: two transposed LDS reads).
+// The weights enter the value product as bf16 (2^-9 relative each, against the 2^-9 of the output's own rounding) and their sum is taken of the rounded ones, so that they still add up to
+// one; scores, references, sums and accumulators are fp32.
+// Measured, 32 heads over 8 key heads of 128: 64 sequences x 16 rows over 8192 shared keys 151 us = 910 TFLOP/s (a large matrix product of the library reaches 1192 on the same card);
+// 64 x 1 row over 1000 own keys 47 us = 5.6 TB/s (a large copy: 4.9, counted both ways).
 #include "../../include/infinisst_hip.h"
 #include "common.h"
 #include "kernels.h"
@@ -17,8 +22,9 @@ typedef __attribute__((ext_vector_type(16))) float f32x16_t;
 typedef __attribute__((ext_vector_type(4))) short s16x4_t;
 typedef __attribute__((address_space(3))) void* lds_ptr;
 
+#define PA_NW 4                  // waves of a workgroup, two workgroups a CU: the waits of one hide behind the other (eight waves, one a CU: 64 x 16 rows 151 -> 158 us, 64 x 5 rows 78 -> 92)
 #define PA_TILE 32               // keys of a block tile
-#define PA_RAISE 0x1p16f         // sum of a step's weights from which a column's reference exponent is raised
+#define PA_RAISE 0x1p16f         // sum of a lane's weights in a step from which a column's reference is raised
 // Keys and values are read through buffer descriptors that start at a tile's first row: a lane's offset is either its row's (rows lie up to 2^25 bytes apart, 63 of them stay inside the
 // descriptor) or PA_OOB, for which the load returns zeros -- also with the scalar offset of the row group added.
 #define PA_EXTENT 0x7fffffffu
@@ -98,8 +104,10 @@ __device__ void add_keys(const isst_prefix_attn& a, const PrefixPlan& p, const K
 }
 
 // ---------------------------------------------------------------------------------------------------------------- block role
-// columns [c0, c0 + 32 NW) against the key tiles of span `split` of `splits`.  A wave owns 32 columns.  K and V tiles go from registers into a ring of three LDS stages; the score product of
-// the next tile is issued with this tile's exponentials, so that the matrix pipe and the vector ALU work at the same time (two workgroups per CU: 256 registers a lane).
+// columns [c0, c0 + 32 NW) against the key tiles of span `split` of `splits`.  A wave owns 32 columns.  Key and value tiles arrive by LDS-DMA in rings of four stages (64 KB: two workgroups a
+// CU), two tiles between barriers.  The matrix instructions of a tile are 512 cycles of the matrix pipe, its vector instructions 440 cycles of issue: one after the other the two waves of a
+// SIMD reached 750 TFLOP/s (tiles through registers, one a barrier), the same with LDS-DMA; exponentials between the matrix instructions of the neighbouring tiles 840; two tiles a barrier and
+// no 64-bit address arithmetic per tile 910, with the matrix pipe busy half of the time.
 template <int D, int NW>
 __device__ __forceinline__ void block_role(const isst_prefix_attn& a, const PrefixPlan& p, char* lds, const KeySpan& w, int c0, int split, int splits, int slot) {
     constexpr int ROWB = 2 * D, CH = D / 8, LOADS = PA_TILE * CH / (NW * 64), RSTEP = NW * 64 / CH, QS = D / 16, DT = D / 32, STAGE = PA_TILE * ROWB;
@@ -202,7 +210,7 @@ __device__ __forceinline__ void block_role(const isst_prefix_attn& a, const Pref
     // Step i: the scores of tile i are in sc and become weights; on the way the values of tile i - 1, whose weights are in pf, are added and the scores of tile i + 1 are computed.
     // A column's reference m is the maximum of its first tile (and of its edge tiles): weights are exponentials against it, bf16 and fp32 hold them to 2^127, and no bit is lost by their
     // size.  So other maxima are not looked for -- that and the running sum were 100 of the 169 vector instructions of a tile -- and only weights that pass PA_RAISE (or NaN) move m,
-    // before anything of the tile was used.
+    // before anything of the tile was used.  (2^16, so that values up to 2^90 cannot overflow the accumulators; scores have to rise by 11 above a column's first tile to get there.)
     u32x4_t pf[2];
     enum { NONE, WHOLE, EDGE } before = NONE;  // what tile i - 1 was: EDGE, some column did not see some key of it
     auto ref = [&]() { return m == -INFINITY ? 0.f : -m; };
@@ -360,7 +368,8 @@ __device__ __forceinline__ void block_role(const isst_prefix_attn& a, const Pref
 }
 
 // ---------------------------------------------------------------------------------------------------------------- span role
-// columns [c0, c0 + 16 NQ) over all their keys; the waves of `splits` workgroups take 32 keys at a time each and are joined at the end
+// columns [c0, c0 + 16 NQ) over all their keys; the waves of `splits` workgroups take 32 keys at a time each and are joined at the end.  Keys go straight to registers in the layout of the
+// product, values by LDS-DMA into two tiles of the wave's own (no barrier), both a step ahead.  64 x 1 row over 1000 own keys: 5.6 TB/s.
 template <int D, int NW, int NQ>
 __device__ __forceinline__ void span_role(const isst_prefix_attn& a, const PrefixPlan& p, char* lds, const KeySpan& w, int c0, int split, int splits, int slot) {
     constexpr int ROWB = 2 * D, CH = D / 8, VL = 32 * CH / 64, VR = 64 / CH, QS = D / 32, NT = D / 16;
@@ -575,7 +584,8 @@ __device__ __forceinline__ void span_role(const isst_prefix_attn& a, const Prefi
 
 template <int D, int NW, int NQ>
 __global__ __launch_bounds__(NW * 64, 2) void prefix_attn_partial_kernel(isst_prefix_attn a, PrefixPlan p) {
-    constexpr int BLOCK_LDS = 4 * 2 * PA_TILE * 2 * D, SPAN_LDS = NW * 32 * D * 4 + NW * 16 * NQ * 8 + 16;  // (ring of three stages; the turned accumulators of a block, the value tiles and the join of a span)
+    constexpr int BLOCK_LDS = 4 * 2 * PA_TILE * 2 * D, SPAN_LDS = NW * 32 * D * 4 + NW * 16 * NQ * 8 + 16;  // (two rings of four stages, or the turned accumulators of a block; the value tiles, or the joined accumulators, and the statistics of a span.  ONE object: with a second one
+    // the compiler would wait for every LDS-DMA in front of every read)
     __shared__ __attribute__((aligned(16))) char lds[BLOCK_LDS > SPAN_LDS ? BLOCK_LDS : SPAN_LDS];
     // workgroup i runs on XCD i % 8 (each with an L2 of its own): the column tiles that read the same keys are neighbours on one XCD
     const bool prefix = (int)blockIdx.x < p.prefix_units;
@@ -653,21 +663,18 @@ __global__ __launch_bounds__(256) void prefix_attn_join_kernel(isst_prefix_attn 
 }
 
 // ---------------------------------------------------------------------------------------------------------------- host
-#ifndef PA_NW
-#define PA_NW 4
-#endif
-#ifndef PA_TAU
+// the launch's model, in microseconds: a tile of 128 columns in a full chip (128-wide heads), and what a unit costs beside its tiles (start, turning and storing its accumulators)
 #define PA_TAU 1.0
-#endif
-#ifndef PA_FIX
 #define PA_FIX 5.0
-#endif
+#define PA_MAX_UNITS (1L << 22)
 static int ceil_div(long a, long b) { return (int)((a + b - 1) / b); }
-// most columns of a sequence that the launch is shaped for
+// most columns of a sequence that the launch is shaped for (of the hint, or the mean: a longer sequence walks on in its units)
 static long own_columns(const isst_prefix_attn& a) {
     const int rows = a.row_starts ? (a.max_rows ? a.max_rows : ceil_div(a.rows, a.seqs)) : a.rows / a.seqs;
     return (long)(rows > 0 ? rows : 1) * (a.heads / a.kv_heads);
 }
+// Columns of a span: 16, or 32 where a sequence (or the batch, against the prefix) has 17 to 32: the keys are then read once (64 x 5 rows of 4 heads over 500 own keys: 39 us, as two spans of 16
+// 44).  From 33 on the block role: at 40 columns 60 us against 58 as three spans, at 64 64 against 64, at 88 and more faster
 static int span_nq(const isst_prefix_attn& a) {
     const long own = a.tail_cap > 0 ? own_columns(a) : 0, all = a.prefix_len > 0 ? (long)a.rows * (a.heads / a.kv_heads) : 0;
     return (own > 16 && own <= 32) || (all > 16 && all <= 32) ? 2 : 1;
@@ -684,6 +691,7 @@ static PrefixPlan plan(const isst_prefix_attn& a) {
         p.own_block = oc > 32;
         p.own_tiles = ceil_div(oc, p.own_block ? width : 16 * nq);
         const long groups = (long)a.seqs * a.kv_heads, keys = p.own_block ? PA_TILE : 32 * PA_NW;
+        while (p.own_tiles > 1 && groups * p.own_tiles > PA_MAX_UNITS) p.own_tiles = (p.own_tiles + 1) / 2;  // (a grid ends at 2^32 threads: the units walk on)
         p.own_splits = 1;
         while (p.own_splits < 8 && groups * p.own_tiles * p.own_splits * 2 <= room && p.own_splits * 2 <= ceil_div(a.tail_cap, (p.own_block ? 4 : 2) * keys)) p.own_splits *= 2;
         p.own_units = p.own_tiles * 8 * ceil_div(groups * p.own_splits, 8);
@@ -693,10 +701,10 @@ static PrefixPlan plan(const isst_prefix_attn& a) {
         p.prefix_block = cols > 32;
         p.prefix_tiles = p.prefix_block ? ceil_div(cols, width) : 1;
         if (p.prefix_block) {
-            // key spans: the rounds of the chip that the units take (with the own keys' units filling what a last round leaves) + what their partial results cost
+            // Key spans: the rounds of the chip that the units take (with the own keys' units filling what a last round leaves) + what their partial results cost
             const int tiles = ceil_div(a.prefix_len, PA_TILE), groups = a.kv_heads * p.prefix_tiles;
             double best = 1e30;
-            for (int s = 1; s <= PA_MAX_SLOTS - 8 && s <= tiles; ++s) {
+            for (int s = 1; s <= PA_MAX_SLOTS - 8 && s <= tiles && (s == 1 || (long)groups * s <= PA_MAX_UNITS); ++s) {
                 const int per = ceil_div(tiles, s);
                 if (ceil_div(tiles, per) != s) continue;
                 const double dur = per * PA_TAU * (a.head_dim / 128.0) + PA_FIX, units = (double)groups * s;
