@@ -755,12 +755,6 @@ def _expect(what: str, dev: int, name: str, t: torch.Tensor, dtype: torch.dtype,
 
 def _row_strides(what: str, name: str, t: torch.Tensor):
     """Strides of all dims but the last (0 where a dim has no second entry), for rows the kernels read 16 bytes at a time."""
-    st = t.stride()
-    bits = 0
-    for s in st[:-1]:
-        bits |= s
-    if st[-1] == 1 and not bits & 7 and not t.data_ptr() & 15:
-        return st[:-1]
     if t.numel() == 0:
         return (0,) * (t.dim() - 1)
     st = tuple(s if n > 1 else 0 for s, n in zip(t.stride()[:-1], t.shape[:-1]))
@@ -773,7 +767,7 @@ def _launch(what: str, dev: int, workspace_bytes: int, call):
     """call(workspace pointer, bytes, stream) on the current stream of `dev`; the workspace is the caching allocator's, i.e. ordered by that stream."""
     if workspace_bytes < 0:
         raise IsstError(f"{what}: bad arguments ({workspace_bytes})")
-    if dev != torch.cuda.current_device():
+    if dev != torch._C._cuda_getDevice():
         with torch.cuda.device(dev):
             return _launch(what, dev, workspace_bytes, call)
     ws = torch.empty(workspace_bytes, dtype=torch.uint8, device=dev) if workspace_bytes else None
@@ -807,15 +801,20 @@ def op_prefix_attention(q: torch.Tensor, k_prefix: torch.Tensor, v_prefix: torch
     if row_starts is not None:
         _expect(what, dev, "row_starts", row_starts, torch.int32, (seqs + 1,))
     if out is None:
-        out = torch.empty((rows, heads, D), dtype=bf, device=dev)
+        out = q.new_empty((rows, heads, D))
     else:
         _expect(what, dev, "out", out, bf, (rows, heads, D), False)
     if D not in (64, 128) or kv < 1 or heads < 1 or heads % kv or (rows and not seqs) or (row_starts is None and seqs and rows % seqs) or max_rows < 0:
         raise IsstError(f"{what}: {rows} rows of {seqs} sequences, {heads} heads on {kv} key heads of {D} (max_rows {max_rows}) are not supported")
-    a = _PrefixAttn(q.data_ptr(), k_prefix.data_ptr(), v_prefix.data_ptr(), k_tail.data_ptr(), v_tail.data_ptr(), tail_lens.data_ptr(),
-                    None if row_starts is None else row_starts.data_ptr(), out.data_ptr(), *_row_strides(what, "q", q), *_row_strides(what, "out", out),
-                    *_row_strides(what, "k_prefix", k_prefix), *_row_strides(what, "v_prefix", v_prefix), *_row_strides(what, "k_tail", k_tail),
-                    *_row_strides(what, "v_tail", v_tail), rows, seqs, max_rows, heads, kv, D, P, cap, D ** -0.5 if scale is None else scale)
+    pq, po, pkp, pvp, pkt, pvt = q.data_ptr(), out.data_ptr(), k_prefix.data_ptr(), v_prefix.data_ptr(), k_tail.data_ptr(), v_tail.data_ptr()
+    (q0, q1, q2), (o0, o1, o2), (kp0, kp1, kp2), (vp0, vp1, vp2) = q.stride(), out.stride(), k_prefix.stride(), v_prefix.stride()
+    (kt0, kt1, kt2, kt3), (vt0, vt1, vt2, vt3) = k_tail.stride(), v_tail.stride()
+    if (q2 != 1 or o2 != 1 or kp2 != 1 or vp2 != 1 or kt3 != 1 or vt3 != 1 or (q0 | q1 | o0 | o1 | kp0 | kp1 | vp0 | vp1 | kt0 | kt1 | kt2 | vt0 | vt1 | vt2) & 7
+            or (pq | po | pkp | pvp | pkt | pvt) & 15):  # (mostly dims of one entry or none, whose strides do not count)
+        (q0, q1), (o0, o1), (kp0, kp1), (vp0, vp1), (kt0, kt1, kt2), (vt0, vt1, vt2) = (
+            _row_strides(what, n, t) for n, t in (("q", q), ("out", out), ("k_prefix", k_prefix), ("v_prefix", v_prefix), ("k_tail", k_tail), ("v_tail", v_tail)))
+    a = _PrefixAttn(pq, pkp, pvp, pkt, pvt, tail_lens.data_ptr(), None if row_starts is None else row_starts.data_ptr(), po, q0, q1, o0, o1, kp0, kp1, vp0, vp1, kt0, kt1, kt2,
+                    vt0, vt1, vt2, rows, seqs, max_rows, heads, kv, D, P, cap, D ** -0.5 if scale is None else scale)
     ref = C.byref(a)
     _launch(what, dev, lib.isst_op_prefix_attention_workspace(ref), lambda ws, n, st: lib.isst_op_prefix_attention(ref, ws, n, st))
     return out
@@ -832,19 +831,26 @@ def op_gemm_lora(x: torch.Tensor, packed: torch.Tensor, N: int, down: torch.Tens
         raise IsstError(f"{what}: x (M, K), down (n, rank, K), got {tuple(x.shape)}, {tuple(down.shape)}")
     bf = torch.bfloat16
     (M, K), (n, rank, _) = x.shape, down.shape
-    _expect(what, dev, "x", x, bf, (M, K), False)
-    _expect(what, dev, "packed", packed, bf, ((N + 15) // 16 * 16 * K,))
-    _expect(what, dev, "down", down, bf, (n, rank, K))
-    _expect(what, dev, "up", up, bf, (n, N, rank))
-    _expect(what, dev, "scales", scales, torch.float32, (n,))
-    _expect(what, dev, "row_adapter", row_adapter, torch.int32, (M,))
+    image = (N + 15) // 16 * 16 * K
+    if not (x.dtype is bf and packed.dtype is bf and down.dtype is bf and up.dtype is bf and scales.dtype is torch.float32 and row_adapter.dtype is torch.int32
+            and packed.shape == (image,) and up.shape == (n, N, rank) and scales.shape == (n,) and row_adapter.shape == (M,)
+            and packed.get_device() == dev and down.get_device() == dev and up.get_device() == dev and scales.get_device() == dev and row_adapter.get_device() == dev
+            and packed.is_contiguous() and down.is_contiguous() and up.is_contiguous() and scales.is_contiguous() and row_adapter.is_contiguous()):
+        _expect(what, dev, "x", x, bf, (M, K), False)
+        _expect(what, dev, "packed", packed, bf, (image,))
+        _expect(what, dev, "down", down, bf, (n, rank, K))
+        _expect(what, dev, "up", up, bf, (n, N, rank))
+        _expect(what, dev, "scales", scales, torch.float32, (n,))
+        _expect(what, dev, "row_adapter", row_adapter, torch.int32, (M,))
     if out is None:
-        out = torch.empty((M, N), dtype=bf, device=dev)
+        out = x.new_empty((M, N))
     else:
         _expect(what, dev, "out", out, bf, (M, N), False)
         if (N > 1 and out.stride(1) != 1) or (M > 1 and out.stride(0) < N):
             raise IsstError(f"{what}: rows of out must be contiguous and apart (strides {out.stride()})")
-    (lda,) = _row_strides(what, "x", x)
+    lda = x.stride(0)
+    if x.stride(1) != 1 or lda & 7:
+        (lda,) = _row_strides(what, "x", x)
     if M > 1 and lda < K:
         raise IsstError(f"{what}: rows of x overlap (strides {x.stride()})")
     _launch(what, dev, lib.isst_op_gemm_lora_workspace(M, N, K, rank, n),
@@ -878,8 +884,7 @@ def op_verify_drafts(target: torch.Tensor, drafts: torch.Tensor, n_drafts: Optio
     t_st, d_st = target.stride(), (0, 0, 1) if draft_scores is None else draft_scores.stride()
     if V > 1 and (t_st[2] != 1 or d_st[2] != 1):
         raise IsstError(f"{what}: rows of the scores must be contiguous (strides {t_st}, {d_st})")
-    tokens = torch.empty((B, K + 1), dtype=torch.int32, device=dev)
-    counts = torch.empty((B,), dtype=torch.int32, device=dev)
+    tokens, counts = drafts.new_empty((B, K + 1)), drafts.new_empty((B,))
     ptr = lambda t: None if t is None else t.data_ptr()
     _launch(what, dev, lib.isst_op_verify_drafts_workspace(B, K, V),
             lambda ws, n, st: lib.isst_op_verify_drafts(target.data_ptr(), t_st[0], t_st[1], ptr(draft_scores), d_st[0], d_st[1], drafts.data_ptr(), ptr(n_drafts), ptr(uniforms),
