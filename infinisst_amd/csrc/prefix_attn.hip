@@ -670,7 +670,7 @@ __global__ __launch_bounds__(256) void prefix_attn_join_kernel(isst_prefix_attn 
 static int ceil_div(long a, long b) { return (int)((a + b - 1) / b); }
 // most columns of a sequence that the launch is shaped for (of the hint, or the mean: a longer sequence walks on in its units)
 static long own_columns(const isst_prefix_attn& a) {
-    const int rows = a.row_starts ? (a.max_rows ? a.max_rows : ceil_div(a.rows, a.seqs)) : a.rows / a.seqs;
+    const int rows = a.row_starts ? (a.max_rows ? min(a.max_rows, a.rows) : ceil_div(a.rows, a.seqs)) : a.rows / a.seqs;
     return (long)(rows > 0 ? rows : 1) * (a.heads / a.kv_heads);
 }
 // Columns of a span: 16, or 32 where a sequence (or the batch, against the prefix) has 17 to 32: the keys are then read once (64 x 5 rows of 4 heads over 500 own keys: 39 us, as two spans of 16

@@ -229,6 +229,75 @@ def test_prefix_attention_offsets_past_32_bits():
     attn_check(E.op_prefix_attention(q, kp2, vp2, kt2, vt2, ln, st, 2), o, A)
 
 
+@pytest.mark.parametrize("R,H,KV,D", [(33, 1, 1, 128), (150, 4, 4, 64), (400, 8, 4, 128)])
+def test_prefix_attention_every_number_of_tiles(R, H, KV, D):
+    """Prefixes from one key to past four tiles of every remainder that matters, by columns of many rows at once (whatever spans the launch cuts them into)."""
+    for P in list(range(1, 5)) + list(range(30, 36)) + list(range(62, 67)) + list(range(94, 100)) + [127, 128, 129, 160, 161, 191, 192, 193, 224, 225, 257, 289, 320, 353, 385]:
+        q, kp, vp, kt, vt, ln, st = attn_inputs(P, [R], [0], H, KV, D, P, 8)
+        print(R, P, flush=True)
+        got = E.op_prefix_attention(q, kp, vp, kt[:, :, :0], vt[:, :, :0], ln, st, R).cpu().double()
+        qd, k, v = (t.cpu().double() for t in (q, kp, vp))
+        w = torch.softmax((qd.view(R, KV, H // KV, D).permute(1, 0, 2, 3).reshape(KV, -1, D) @ k.transpose(1, 2)) * D ** -0.5, -1)
+        back = lambda x: x.view(KV, R, H // KV, D).permute(1, 0, 2, 3).reshape(R, H, D)
+        attn_check(got, back(w @ v), back(w @ v.abs()), f"P {P}")
+
+
+@pytest.mark.parametrize("rows", [9, 40, 70])
+def test_prefix_attention_own_keys_of_every_length(rows):
+    """Own keys of one sequence among others, from its rows alone to past four tiles: causal edges at every place of a tile."""
+    for L in list(range(rows, rows + 36, 5)) + [95, 96, 97, 127, 128, 129, 150, 161, 193, 230, 260]:
+        counts, lens = [1, rows, 2], [L // 2 + 1, max(L, rows), 3]
+        q, kp, vp, kt, vt, ln, st = attn_inputs(L, counts, lens, 8, 2, 128, 37, 272)
+        o, A = attn_ref(q, kp, vp, kt, vt, ln, st)
+        print(rows, L, flush=True)
+        attn_check(E.op_prefix_attention(q, kp, vp, kt, vt, ln, st, rows), o, A, f"{rows} rows, {L} keys")
+
+
+def test_prefix_attention_long_prefix_few_rows_and_wild_hints():
+    q, kp, vp, kt, vt, ln, st = attn_inputs(31, [1, 2], [5, 60], 4, 1, 128, 60001, 64)
+    o, A = attn_ref(q, kp, vp, kt, vt, ln, st)
+    for hint in (0, 2, 10 ** 9):
+        attn_check(E.op_prefix_attention(q, kp, vp, kt, vt, ln, st, hint), o, A, f"max_rows {hint}")
+    rows, lens = [150] + [1] * 30, [700] + [20] * 30  # one sequence far above the mean, which sizes the launch without a hint
+    q, kp, vp, kt, vt, ln, st = attn_inputs(32, rows, lens, 4, 2, 64, 100, 700)
+    o, A = attn_ref(q, kp, vp, kt, vt, ln, st)
+    for hint in (0, 1, 150):
+        attn_check(E.op_prefix_attention(q, kp, vp, kt, vt, ln, st, hint), o, A, f"max_rows {hint}")
+
+
+def test_prefix_attention_in_place_and_one_key_for_all():
+    """The output in the place of the queries; a prefix whose keys are one row repeated (stride 0)."""
+    rows, lens = [2, 40], [9, 50]
+    q, kp, vp, kt, vt, ln, st = attn_inputs(33, rows, lens, 8, 2, 128, 90, 64)
+    want = E.op_prefix_attention(q, kp, vp, kt, vt, ln, st, 40)
+    again = q.clone()
+    assert E.op_prefix_attention(again, kp, vp, kt, vt, ln, st, 40, out=again) is again and torch.equal(again, want)
+    one_k, one_v = kp[:, :1].expand(-1, 90, -1), vp[:, :1].expand(-1, 90, -1)
+    o, A = attn_ref(q, one_k, one_v, kt, vt, ln, st)
+    attn_check(E.op_prefix_attention(q, one_k, one_v, kt, vt, ln, st, 40), o, A)
+
+
+def test_prefix_attention_without_any_slot():
+    """No prefix and no room for own keys: every row of a sequence is zero, the others stay."""
+    z = lambda *s: torch.empty(*s, dtype=BF, device=DEV)
+    q, out = torch.randn(5, 4, 128, device=DEV).to(BF), torch.full((5, 4, 128), 3.0, dtype=BF, device=DEV)
+    st = torch.tensor([1, 3, 4], dtype=torch.int32, device=DEV)
+    E.op_prefix_attention(q, z(2, 0, 128), z(2, 0, 128), z(2, 2, 0, 128), z(2, 2, 0, 128), torch.tensor([7, 0], dtype=torch.int32, device=DEV), st, 2, out=out)
+    assert out[:, 0, 0].tolist() == [3.0, 0.0, 0.0, 0.0, 3.0] and bool((out[1:4] == 0).all())
+
+
+def test_prefix_attention_values_of_any_size():
+    """Values up to 2^90 behind scores that rise by 14 in between (fp32 accumulators end at 2^128)."""
+    rows, lens = [3, 30], [90, 60]
+    q, kp, vp, kt, vt, ln, st = attn_inputs(34, rows, lens, 4, 2, 128, 300, 96)
+    kp[:, 200:, 0], q[..., 0] = 20.0, 8.0
+    for f in (2.0 ** 90, 2.0 ** -90):
+        vp2, vt2 = vp * f, vt * f
+        o, A = attn_ref(q, kp, vp2, kt, vt2, ln, st)
+        got = E.op_prefix_attention(q, kp, vp2, kt, vt2, ln, st, 30).cpu().double()
+        assert bool(((got - o).abs() <= U_BF * o.abs() + (U_BF + 2.0 ** -11) * A).all())  # (scores up to 34, not 20: 2^-12 becomes 2^-11)
+
+
 # ---------------------------------------------------------------------------------------------------------------- adapters
 def lora_inputs(seed, M, N, K, rank, n, ids):
     g = torch.Generator().manual_seed(seed)
@@ -304,6 +373,14 @@ def test_gemm_lora_strided():
     ref = lora_run(x, W, down, up, scales, ids)
     got = E.op_gemm_lora(wide[:, K:2 * K], E.op_pack_weight(W.to(DEV)), N, down.to(DEV), up.to(DEV), scales.to(DEV), ids.to(DEV), out=out[:, 8:8 + N])
     assert torch.equal(got, ref) and bool((out[:, :8] == 5.0).all()) and bool((out[:, 8 + N:] == 5.0).all())
+
+
+def test_gemm_lora_in_place():
+    M, K, rank, n = 70, 256, 16, 4
+    x, W, down, up, scales, ids = lora_inputs(3, M, K, K, rank, n, [m % 5 - 1 for m in range(M)])
+    want, xd = lora_run(x, W, down, up, scales, ids), x.to(DEV)
+    E.op_gemm_lora(xd, E.op_pack_weight(W.to(DEV)), K, down.to(DEV), up.to(DEV), scales.to(DEV), ids.to(DEV), out=xd)
+    assert torch.equal(xd, want)
 
 
 # ---------------------------------------------------------------------------------------------------------------- drafts
@@ -430,6 +507,22 @@ def test_verify_drafts_bad_rows_name_their_stream_only():
     drafts[:, 1:] = 10 ** 9
     assert (verify_ref(t, drafts, n, q, u)[1] == 1).all()
     verify_same((t, drafts, n, q, u))
+
+
+def test_verify_drafts_rows_behind_the_drafts_do_not_matter():
+    B, K, V = 8, 5, 4500
+    for kind in ("scores", "bare", "greedy"):
+        t, drafts, n, q, u = verify_inputs(12, B, K, V)
+        n[:] = np.arange(B) % (K + 1)
+        drafts = np.where(np.random.default_rng(3).random((B, K)) < 0.8, t[:, :K].argmax(-1), drafts).astype(np.int32)
+        if kind == "scores":  # a draft that is sure of its token, as the target is: accepted mostly
+            t[np.arange(B)[:, None], np.arange(K), drafts] += 20.0
+            q[np.arange(B)[:, None], np.arange(K), drafts] += 18.0
+        for b in range(B):
+            t[b, n[b] + 1:], q[b, n[b]:], drafts[b, n[b]:] = np.nan, np.inf, -5
+        want = verify_ref(t, drafts, n, q if kind == "scores" else None, None if kind == "greedy" else u)
+        assert (want[1] > 0).all() and (want[1] == n + 1).sum() >= 2
+        verify_same((t, drafts, n, q if kind == "scores" else None, None if kind == "greedy" else u))
 
 
 def test_verify_drafts_strided_scores():

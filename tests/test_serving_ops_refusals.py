@@ -35,6 +35,16 @@ def test_prefix_attention_refuses(lib, bad):
     assert lib.isst_op_prefix_attention(C.byref(a), FAKE, 1 << 40, None) == -1
 
 
+def test_prefix_attention_size_limits(lib):
+    """rows * heads <= 2^26, seqs * kv_heads <= 2^22, heads <= 2^15, a key's stride <= 2^24: the limits themselves are taken, one more is not."""
+    ws = lambda **kw: lib.isst_op_prefix_attention_workspace(C.byref(attn(**kw)))
+    assert ws(rows=1 << 24) >= (1 << 26) * (128 * 4 + 8) and ws(rows=(1 << 24) + 1) == -1
+    assert ws(seqs=1 << 21, max_rows=1 << 30) > 0 and ws(seqs=(1 << 21) + 1) == -1
+    assert ws(heads=1 << 15, kv_heads=1, q_row=1 << 22, out_row=1 << 22) > 0 and ws(heads=1 << 16, kv_heads=1, q_row=1 << 23, out_row=1 << 23) == -1
+    for key in ("kp_key", "vp_key", "kt_key", "vt_key"):
+        assert ws(**{key: 1 << 24}) > 0 and ws(**{key: (1 << 24) + 8}) == -1 and ws(**{key: -8}) == -1
+
+
 def test_prefix_attention_workspace(lib):
     assert lib.isst_op_prefix_attention(None, None, 0, None) == -1 and lib.isst_op_prefix_attention_workspace(None) == -1
     a = attn()
