@@ -2,10 +2,10 @@
 // p, q = softmax of fp32 score rows.  Everything behind the scores is in 64 bits: the outcome of a comparison or of a draw must not depend on the order of a sum, and with
 // 32-bit probabilities the borders of the inverse CDF move by ~1e-8 each -- over 128 k of them one draw in a thousand would land elsewhere.
 //
-// Launch 1 reads every score row once, a workgroup per slice of VF_SLICE entries (maximum and its first index, or sum of exponentials); its floor is that read, and the 64-bit exponential
-// is short enough to hide most of itself behind it.  Drafts with scores need two more: who decides (a workgroup per stream), and what a refused draft leaves over, slice by slice.  The last
+// Launch 1 reads every score row once, a workgroup per slice of VF_SLICE entries (maximum and its first index, or sum of exponentials); its floor is that read, and most of
+// the 64-bit exponentials hides behind it.  Drafts with scores need two more: who decides (a workgroup per stream), and what a refused draft leaves over, slice by slice.  The last
 // launch takes one workgroup per stream: find the slice that the draw falls into from the slice sums, walk that slice.
-// Measured, rows of 128263: 64 streams x 4 drafts with scores 62 us (265 MB: 4.3 TB/s) + decide 4.8 + left over 15.5 + draw 6.8; one stream without scores 6.2 + 7.0, latency all of it (in cycles
+// Measured, rows of 128263: 64 streams x 4 drafts with scores 57 us (265 MB: 4.6 TB/s) + decide 4.8 + left over 14.3 + draw 6.8; one stream without scores 6.2 + 6.6, latency all of it (in cycles
 // of the draw: decide 5400, find the slice 3300, its weights 3200, walk 2600).
 #include "common.h"
 #include "kernels.h"
@@ -20,13 +20,15 @@ struct VerifyStat { double sum; float max; int at; };  // of a slice: sum of exp
 
 typedef float f32x4u_t __attribute__((ext_vector_type(4), aligned(4)));  // (rows start anywhere)
 
-// exp(d) for -700 <= d <= 0: 2^k exp(r), k the nearest whole number to d / ln 2 (added to 1.5 2^52, where it is the low word), |r| <= ln 2 / 2, the Taylor series up to r^10 / 10!.  Its
-// remainder is below 2.2e-13 relative: over 128 k borders of an inverse CDF one draw in 10^7 could land elsewhere for it.  17 instructions, 16 of them in 64 bits (with it and one decision a stream instead of one a slice, 64 streams 120 -> 105 us).
+// exp(d) for -700 <= d <= 0: 2^k exp(r), k the nearest whole number to d / ln 2 (added to 1.5 2^52, where it is the low word), |r| <= ln 2 / 2, the polynomial of degree 8 through exp at the
+// Chebyshev nodes of that interval.  Its error is below 1.1e-12 relative (checked against 60 digits on 4001 points): over 128 k borders of an inverse CDF one draw in 10^7 could land elsewhere
+// for it.  The score read is bound by these instructions -- a 64-bit multiply-add an entry is 2.4 us of the 82 that 64 streams x 4 drafts with scores take (Taylor to r^10 / 10!, 2.2e-13: 86 us;
+// degree 9, 2e-14: 84).
 __device__ __forceinline__ double exp_core(double d) {
     const double t = fma(d, 1.4426950408889634074, 0x1.8p52), k = t - 0x1.8p52, r = fma(-k, 0.69314718055994530942, d);
-    double p = 1.0 / 3628800.0;
-    p = fma(p, r, 1.0 / 362880.0); p = fma(p, r, 1.0 / 40320.0); p = fma(p, r, 1.0 / 5040.0); p = fma(p, r, 1.0 / 720.0); p = fma(p, r, 1.0 / 120.0);
-    p = fma(p, r, 1.0 / 24.0); p = fma(p, r, 1.0 / 6.0); p = fma(p, r, 0.5); p = fma(p, r, 1.0); p = fma(p, r, 1.0);
+    double p = 2.487616403756168e-05;
+    p = fma(p, r, 0.00019915866941726544); p = fma(p, r, 0.0013888821677603455); p = fma(p, r, 0.008333266097922691); p = fma(p, r, 0.04166666689095713);
+    p = fma(p, r, 0.16666666891045911); p = fma(p, r, 0.49999999999797934); p = fma(p, r, 0.9999999999797852); p = fma(p, r, 1.0);
     return __hiloint2double(__double2hiint(p) + (__double2loint(t) << 20), __double2loint(p));
 }
 // ... for any d <= 0; under -700 and for NaN (-inf less -inf): 0
