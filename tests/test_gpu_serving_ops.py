@@ -347,6 +347,16 @@ def test_gemm_lora_row_orders(M, N, K, rank, n, spread):
     lora_check(lora_run(*args), *args, what=spread)
 
 
+@pytest.mark.parametrize("rank", [8, 16, 24, 32, 40, 64, 72, 96, 128])
+def test_gemm_lora_many_rows_of_every_rank(rank):
+    """Enough rows and columns for the wide form of the adapter sum (1040 x 1031: 65 x 17 tiles), runs of rows and a changing adapter per row, a column tail, K past one slice."""
+    M, N, n = 1040, 1031, 6
+    for K, ids in ((96, [(m // 22) % (n + 1) - 1 for m in range(M)]), (1056, [(7 * m) % (n + 2) - 1 for m in range(M)])):
+        args = lora_inputs(rank + K, M, N, K, rank, n, ids)
+        print(rank, K, flush=True)
+        lora_check(lora_run(*args), *args, what=f"rank {rank} K {K}")
+
+
 def test_gemm_lora_adapters_do_not_mix():
     """An adapter of NaN / inf weights, a NaN scale and a NaN row reach their own rows only; wild ids mean no adapter."""
     M, N, K, rank, n = 40, 96, 256, 16, 4
