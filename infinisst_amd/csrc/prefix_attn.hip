@@ -11,7 +11,7 @@
 // The weights enter the value product as bf16 (2^-9 relative each, against the 2^-9 of the output's own rounding) and their sum is taken of the rounded ones, so that they still add up to
 // one; scores, references, sums and accumulators are fp32.
 // Measured, 32 heads over 8 key heads of 128: 64 sequences x 16 rows over 8192 shared keys 151 us = 910 TFLOP/s (a large matrix product of the library reaches 1192 on the same card);
-// 64 x 1 row over 1000 own keys 47 us = 5.6 TB/s (a large copy: 4.9, counted both ways).
+// 64 x 1 row over 1000 own keys 47 us = 5.5 TB/s (a large copy: 4.9, counted both ways).
 #include "../../include/infinisst_hip.h"
 #include "common.h"
 #include "kernels.h"
@@ -25,10 +25,6 @@ typedef __attribute__((address_space(3))) void* lds_ptr;
 #define PA_NW 4                  // waves of a workgroup, two workgroups a CU: the waits of one hide behind the other (eight waves, one a CU: 64 x 16 rows 151 -> 158 us, 64 x 5 rows 78 -> 92)
 #define PA_TILE 32               // keys of a block tile
 #define PA_RAISE 0x1p16f         // sum of a lane's weights in a step from which a column's reference is raised
-// Keys and values are read through buffer descriptors that start at a tile's first row: a lane's offset is either its row's (rows lie up to 2^25 bytes apart, 63 of them stay inside the
-// descriptor) or PA_OOB, for which the load returns zeros -- also with the scalar offset of the row group added.
-#define PA_EXTENT 0x7fffffffu
-#define PA_OOB 0x80000000u
 
 // [first, first + n) = the rows of sequence b, clipped to the launch's rows
 __device__ __forceinline__ void seq_rows(const isst_prefix_attn& a, int b, int& first, int& n) {
@@ -80,10 +76,6 @@ __device__ __forceinline__ int tile_off(int row, int ch) {
 __device__ __forceinline__ u32x2_t read_tr(const char* p) {
     return __builtin_bit_cast(u32x2_t, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4_t*)p));
 }
-__device__ __forceinline__ __amdgpu_buffer_rsrc_t key_rsrc(const bf16_t* p) {
-    return __builtin_amdgcn_make_buffer_rsrc(const_cast<bf16_t*>(p), 0, PA_EXTENT, 0x00020000);
-}
-
 // Keys [lo, hi) of one column added to its stored partial result, whose maximum covers them.  Only for tiles that hold inf or NaN values and that some column of a wave does not see
 // whole: in a matrix product 0 x inf would reach the columns that do not see the key.
 template <int D>
@@ -368,36 +360,25 @@ __device__ __forceinline__ void block_role(const isst_prefix_attn& a, const Pref
 }
 
 // ---------------------------------------------------------------------------------------------------------------- span role
-// columns [c0, c0 + 16 NQ) over all their keys; the waves of `splits` workgroups take 32 keys at a time each and are joined at the end.  Keys go straight to registers in the layout of the
-// product, values by LDS-DMA into two tiles of the wave's own (no barrier), both a step ahead.  64 x 1 row over 1000 own keys: 5.6 TB/s.
+// columns [c0, c0 + 16 NQ) over all their keys; the waves of `splits` workgroups take 32 keys at a time each and are joined at the end.  A step's keys and values arrive by LDS-DMA in a buffer of
+// the wave's own (no barrier), go to registers in one piece, and the next step's are asked for before the first product.  64 x 1 row over 1000 own keys: 5.5 TB/s.  (Keys straight to registers in
+// the layout of the product, values in two buffers: 64 x 5 rows 84 -> 82.5 us, 64 x 1 row 46.6 -> 46.0, but 33 x 1..3 rows with heads of 64 16.3 -> 17.3.)
 template <int D, int NW, int NQ>
 __device__ __forceinline__ void span_role(const isst_prefix_attn& a, const PrefixPlan& p, char* lds, const KeySpan& w, int c0, int split, int splits, int slot) {
     constexpr int ROWB = 2 * D, CH = D / 8, VL = 32 * CH / 64, VR = 64 / CH, QS = D / 32, NT = D / 16;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), fr = lane & 15, fq = lane >> 4;
     const int G = a.heads / a.kv_heads, t0 = c0 / G, x0 = c0 % G;
     const int see_least = sees(w, t0), see_most = sees(w, (min(c0 + 16 * NQ, w.ncols) - 1) / G);
-    char* vl = lds + wave * (64 * ROWB);  // two tiles of 32 values, this wave's alone
-    u32x4_t kf[2][QS];
-    const int kstep = (int)w.kstride * 2, vstep = (int)w.vstride * 2;
-    const unsigned koff = fr * kstep + 16 * fq;
-    // values come by LDS-DMA, in front of the keys of the same step: the wait for these is the wait for them
+    char *const kl = lds + wave * (64 * ROWB), *const vl = kl + 32 * ROWB;  // 32 keys and their values, this wave's alone
+    // 1 KB of whole lines an instruction (fragments read from memory are 64 pieces of 16 bytes, a cycle of the L1 cache each); rows behind the last key repeat it
     const int lr = lane / CH;
-    auto fetch_v = [&](int j0, char* dst) {
-        const char* src = reinterpret_cast<const char*>(w.v + j0 * w.vstride);
+    auto fetch = [&](const bf16_t* rows0, long stride, int j0, char* dst) {
+        const char* src = reinterpret_cast<const char*>(rows0 + j0 * stride);
         const int last = see_most - 1 - j0;
 #pragma unroll
         for (int i = 0; i < VL; ++i) {
             const int row = lr + i * VR, lc = tile_off<D>(row, lane % CH) % ROWB;
-            __builtin_amdgcn_global_load_lds((const void*)(src + (unsigned)(min(row, last) * vstep + lc)), (lds_ptr)(dst + 1024 * i), 16, 0, 0);
-        }
-    };
-    auto fetch_k = [&](int j0) {
-        const __amdgpu_buffer_rsrc_t r = key_rsrc(w.k + j0 * w.kstride);
-#pragma unroll
-        for (int t = 0; t < 2; ++t) {
-            const unsigned off = fr < see_most - j0 - 16 * t ? koff : PA_OOB;
-#pragma unroll
-            for (int s = 0; s < QS; ++s) kf[t][s] = __builtin_amdgcn_raw_buffer_load_b128(r, off, 16 * t * kstep + 64 * s, 0);
+            __builtin_amdgcn_global_load_lds((const void*)(src + (unsigned)(min(row, last) * (int)(2 * stride) + lc)), (lds_ptr)(dst + 1024 * i), 16, 0, 0);
         }
     };
     float2* wml = reinterpret_cast<float2*>(lds + NW * 32 * D * 4);  // [NW][16 NQ], behind the value tiles / turned accumulators
@@ -406,7 +387,10 @@ __device__ __forceinline__ void span_role(const isst_prefix_attn& a, const Prefi
     __syncthreads();
     const int step = 32 * NW * splits;
     int j0 = 32 * (split * NW + wave);
-    if (j0 < see_most) { fetch_v(j0, vl); fetch_k(j0); }
+    if (j0 < see_most) {
+        fetch(w.k, w.kstride, j0, kl);
+        fetch(w.v, w.vstride, j0, vl);
+    }
 
     int limit[NQ];
     u32x4_t qf[NQ][QS];
@@ -428,10 +412,25 @@ __device__ __forceinline__ void span_role(const isst_prefix_attn& a, const Prefi
     }
     const float c2 = a.scale * 1.44269504088896340736f;
     bool first_step = true;
-    int turn = 0;
     for (; j0 < see_most; j0 += step) {
-        const bool more = j0 + step < see_most;
-        char* const vt = vl + (turn & 1) * (32 * ROWB);
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        bf16x8_t kf[2][QS], vf[NT];
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+            for (int s = 0; s < QS; ++s) kf[t][s] = __builtin_bit_cast(bf16x8_t, *reinterpret_cast<const u32x4_t*>(kl + tile_off<D>(16 * t + fr, 4 * s + fq)));
+        const int vrow = 4 * fq + ((lane >> 2) & 3), vch = (lane & 3) >> 1, vb8 = 8 * (lane & 1);
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+            const u32x2_t v1 = read_tr(vl + tile_off<D>(vrow, 2 * t + vch) + vb8), v2 = read_tr(vl + tile_off<D>(16 + vrow, 2 * t + vch) + vb8);
+            vf[t] = __builtin_bit_cast(bf16x8_t, (u32x4_t){v1.x, v1.y, v2.x, v2.y});
+        }
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // (all of the step is in registers: the next one may arrive)
+        __builtin_amdgcn_sched_barrier(0);
+        if (j0 + step < see_most) {
+            fetch(w.k, w.kstride, j0 + step, kl);
+            fetch(w.v, w.vstride, j0 + step, vl);
+        }
         __builtin_amdgcn_sched_barrier(0);
         f32x4_t sc[NQ][2];
 #pragma unroll
@@ -440,24 +439,8 @@ __device__ __forceinline__ void span_role(const isst_prefix_attn& a, const Prefi
             for (int t = 0; t < 2; ++t) {
                 sc[n][t] = (f32x4_t){0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-                for (int s = 0; s < QS; ++s)
-                    sc[n][t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, kf[t][s]), __builtin_bit_cast(bf16x8_t, qf[n][s]), sc[n][t], 0, 0, 0);
+                for (int s = 0; s < QS; ++s) sc[n][t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf[t][s], __builtin_bit_cast(bf16x8_t, qf[n][s]), sc[n][t], 0, 0, 0);
             }
-        __builtin_amdgcn_sched_barrier(0);
-        const int vrow = 4 * fq + ((lane >> 2) & 3), vch = (lane & 3) >> 1, vb8 = 8 * (lane & 1);
-        bf16x8_t vf[NT];
-#pragma unroll
-        for (int t = 0; t < NT; ++t) {
-            const u32x2_t v1 = read_tr(vt + tile_off<D>(vrow, 2 * t + vch) + vb8), v2 = read_tr(vt + tile_off<D>(16 + vrow, 2 * t + vch) + vb8);
-            vf[t] = __builtin_bit_cast(bf16x8_t, (u32x4_t){v1.x, v1.y, v2.x, v2.y});
-        }
-        __builtin_amdgcn_sched_barrier(0);
-        if (more) {
-            fetch_v(j0 + step, vl + (~turn & 1) * (32 * ROWB));
-            fetch_k(j0 + step);
-        }
-        ++turn;
-        __builtin_amdgcn_sched_barrier(0);
         const bool edge = j0 + 32 > see_least;  // some column does not see some key of this step
         auto raise = [&]() {  // m becomes the maximum of what it covers and of these scores
 #pragma unroll
@@ -517,9 +500,9 @@ __device__ __forceinline__ void span_role(const isst_prefix_attn& a, const Prefi
         for (int n = 0; n < NQ; ++n) l[n] += sum[n];
         if (edge) {
             bool ill = false;  // inf or NaN among the values of a step that not every column sees whole
-#pragma unroll 1
-            for (int i = 0; i < VL; ++i) {
-                const u32x4_t v = *reinterpret_cast<const u32x4_t*>(vt + 1024 * i + 16 * lane);
+#pragma unroll
+            for (int t = 0; t < NT; ++t) {
+                const u32x4_t v = __builtin_bit_cast(u32x4_t, vf[t]);
 #pragma unroll
                 for (int w = 0; w < 4; ++w) ill |= (v[w] & 0x7f80u) == 0x7f80u || (v[w] & 0x7f800000u) == 0x7f800000u;
             }
