@@ -600,6 +600,7 @@ __global__ __launch_bounds__(NW * 64, 2) void prefix_attn_partial_kernel(isst_pr
 
 // Joins the slots of a (row, head), D / 4 lanes each.  Bound by latency: the statistics of all slots come in one load (lane i: slot i), the accumulators eight slots at a time.
 #define PA_MAX_SLOTS 32
+#define PA_OWN_SLOTS 8  // of them, at most for the own keys where there is a prefix
 template <int D>
 __global__ __launch_bounds__(256) void prefix_attn_join_kernel(isst_prefix_attn a, PrefixPlan p) {
     constexpr int L4 = D / 4, E = PA_MAX_SLOTS / L4;
@@ -676,7 +677,8 @@ static PrefixPlan plan(const isst_prefix_attn& a) {
         const long groups = (long)a.seqs * a.kv_heads, keys = p.own_block ? PA_TILE : 32 * PA_NW;
         while (p.own_tiles > 1 && groups * p.own_tiles > PA_MAX_UNITS) p.own_tiles = (p.own_tiles + 1) / 2;  // (a grid ends at 2^32 threads: the units walk on)
         p.own_splits = 1;
-        while (p.own_splits < 8 && groups * p.own_tiles * p.own_splits * 2 <= room && p.own_splits * 2 <= ceil_div(a.tail_cap, (p.own_block ? 4 : 2) * keys)) p.own_splits *= 2;
+        const int most = a.prefix_len > 0 ? PA_OWN_SLOTS : PA_MAX_SLOTS;  // (one row over 100000 own keys: 8 spans 139 us, 32 83)
+        while (p.own_splits < most && groups * p.own_tiles * p.own_splits * 2 <= room && p.own_splits * 2 <= ceil_div(a.tail_cap, (p.own_block ? 4 : 2) * keys)) p.own_splits *= 2;
         p.own_units = p.own_tiles * 8 * ceil_div(groups * p.own_splits, 8);
         own_us = (double)groups * p.own_tiles * (p.own_block ? a.tail_cap / 2 / (double)PA_TILE * PA_TAU : a.tail_cap / 2 * (4.0 * a.head_dim) / (20e3 * PA_NW / 8));
     }
@@ -687,7 +689,7 @@ static PrefixPlan plan(const isst_prefix_attn& a) {
             // Key spans: the rounds of the chip that the units take (with the own keys' units filling what a last round leaves) + what their partial results cost
             const int tiles = ceil_div(a.prefix_len, PA_TILE), groups = a.kv_heads * p.prefix_tiles;
             double best = 1e30;
-            for (int s = 1; s <= PA_MAX_SLOTS - 8 && s <= tiles && (s == 1 || (long)groups * s <= PA_MAX_UNITS); ++s) {
+            for (int s = 1; s <= PA_MAX_SLOTS - PA_OWN_SLOTS && s <= tiles && (s == 1 || (long)groups * s <= PA_MAX_UNITS); ++s) {
                 const int per = ceil_div(tiles, s);
                 if (ceil_div(tiles, per) != s) continue;
                 const double dur = per * PA_TAU * (a.head_dim / 128.0) + PA_FIX, units = (double)groups * s;
@@ -697,7 +699,7 @@ static PrefixPlan plan(const isst_prefix_attn& a) {
             }
         } else {
             p.prefix_splits = ceil_div(a.prefix_len, 32 * PA_NW);
-            if (p.prefix_splits > PA_MAX_SLOTS - 8) p.prefix_splits = PA_MAX_SLOTS - 8;
+            if (p.prefix_splits > PA_MAX_SLOTS - PA_OWN_SLOTS) p.prefix_splits = PA_MAX_SLOTS - PA_OWN_SLOTS;
         }
         p.prefix_units = p.prefix_tiles * 8 * ceil_div((long)a.kv_heads * p.prefix_splits, 8);
     }

@@ -277,6 +277,29 @@ def test_prefix_attention_in_place_and_one_key_for_all():
     attn_check(E.op_prefix_attention(q, one_k, one_v, kt, vt, ln, st, 40), o, A)
 
 
+@pytest.mark.parametrize("R,L,P,H,KV,D", [(1500, 1500, 0, 4, 2, 128), (1100, 2300, 77, 3, 3, 64)])
+def test_prefix_attention_whole_prompt_of_one_sequence(R, L, P, H, KV, D):
+    """A prompt pass: every row of a long sequence at once, causal over its own keys, beside a sequence of one row."""
+    q, kp, vp, kt, vt, ln, st = attn_inputs(41, [R, 1], [L, 5], H, KV, D, P, L)
+    got = E.op_prefix_attention(q, kp, vp, kt, vt, ln, st, R).cpu().double()
+    qd = q.cpu().double()[:R].view(R, KV, H // KV, D).permute(1, 2, 0, 3)
+    k, v = (torch.cat([x.cpu().double(), y[0, :, :L].cpu().double()], 1) for x, y in ((kp, kt), (vp, vt)))
+    w = qd @ k[:, None].transpose(2, 3) * D ** -0.5
+    w = torch.softmax(w.masked_fill(torch.arange(P + L)[None] > torch.arange(R)[:, None] + P + L - R, -math.inf), -1)
+    back = lambda x: x.permute(2, 0, 1, 3).reshape(R, H, D)
+    attn_check(got[:R], back(w @ v[:, None]), back(w @ v.abs()[:, None]))
+    o, A = attn_ref(q[R:], kp, vp, kt[1:], vt[1:], ln[1:], torch.tensor([0, 1]))
+    attn_check(got[R:], o, A)
+
+
+@pytest.mark.parametrize("D", [64, 128])
+def test_prefix_attention_long_own_keys(D):
+    """One stream's row over tens of thousands of own keys (as many spans as the join takes), and a short one beside it."""
+    q, kp, vp, kt, vt, ln, st = attn_inputs(43, [1, 3], [20011, 9], 4, 2, D, 0, 20011)
+    o, A = attn_ref(q, kp, vp, kt, vt, ln, st)
+    attn_check(E.op_prefix_attention(q, kp, vp, kt, vt, ln, st, 3), o, A)
+
+
 def test_prefix_attention_without_any_slot():
     """No prefix and no room for own keys: every row of a sequence is zero, the others stay."""
     z = lambda *s: torch.empty(*s, dtype=BF, device=DEV)
