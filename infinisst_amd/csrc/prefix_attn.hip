@@ -76,6 +76,14 @@ __device__ __forceinline__ int tile_off(int row, int ch) {
 __device__ __forceinline__ u32x2_t read_tr(const char* p) {
     return __builtin_bit_cast(u32x2_t, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4_t*)p));
 }
+// LDS-DMA from a buffer descriptor at a tile's first row (a lane's offset and the scalar one of its row group together stay below 2^32).  As global loads the compiler would count it as an LDS
+// access that ends in no known order, and wait for ALL fragments in front of the first product: 64 sequences x 16 rows over 8192 keys 168 us, so 160.  (The span role waits for all of a step anyway,
+// and takes global loads: 64 x 1 row 49 us with descriptors, 47 without.)
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t rows_at(const void* p) { return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(p), 0, 0xffffffffu, 0x00020000); }
+__device__ __forceinline__ void dma(const __amdgpu_buffer_rsrc_t& r, char* dst, unsigned lane_offset, unsigned rows_offset) {
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lds_ptr)dst, 16, lane_offset, rows_offset, 0, 0);
+}
+
 // Keys [lo, hi) of one column added to its stored partial result, whose maximum covers them.  Only for tiles that hold inf or NaN values and that some column of a wave does not see
 // whole: in a matrix product 0 x inf would reach the columns that do not see the key.
 template <int D>
@@ -119,17 +127,17 @@ __device__ __forceinline__ void block_role(const isst_prefix_attn& a, const Pref
     // keys of tile i go to key stage i % 4, its values to value stage i % 4, by LDS-DMA: a wave fills 1 KB at a time in lane order, so the swizzle is in which chunk of its row a lane asks
     // for.  Rows behind the last key repeat it.
     const int lr = tid / CH, lc = tile_off<D>(lr, tid % CH) % ROWB;
-    const long krows = RSTEP * 2 * w.kstride, vrows = RSTEP * 2 * w.vstride;  // bytes between the rows of two loads
-    unsigned koff = lr * (int)(2 * w.kstride) + lc, voff = lr * (int)(2 * w.vstride) + lc;
+    const unsigned krows = RSTEP * 2 * (unsigned)w.kstride, vrows = RSTEP * 2 * (unsigned)w.vstride;  // bytes between the rows of two loads
+    const unsigned koff = lr * (int)(2 * w.kstride) + lc, voff = lr * (int)(2 * w.vstride) + lc;
     char *const kring = lds, *const vring = lds + 4 * STAGE;
     auto stage = [&](int i) { return (i & 3) * STAGE; };
     auto fetch = [&](const bf16_t* rows0, long stride, int i, char* stage) {
         const int left = w.keys - (tile0 + i) * PA_TILE;
         if (i >= tiles) return;
-        const char* src = reinterpret_cast<const char*>(rows0 + (tile0 + i) * PA_TILE * stride);
+        const __amdgpu_buffer_rsrc_t src = rows_at(rows0 + (tile0 + i) * PA_TILE * stride);
 #pragma unroll
         for (int k = 0; k < LOADS; ++k)
-            __builtin_amdgcn_global_load_lds((const void*)(src + (unsigned)(min(lr + k * RSTEP, left - 1) * (int)(2 * stride) + lc)), (lds_ptr)(stage + (k * NW + wave) * 1024), 16, 0, 0);
+            dma(src, stage + (k * NW + wave) * 1024, min(lr + k * RSTEP, left - 1) * (int)(2 * stride) + lc, 0);
     };
     fetch(w.k, w.kstride, 0, kring);
     fetch(w.k, w.kstride, 1, kring + STAGE);
@@ -284,16 +292,16 @@ __device__ __forceinline__ void block_role(const isst_prefix_attn& a, const Pref
     const char *ksrc = reinterpret_cast<const char*>(w.k + (tile0 + 3) * PA_TILE * w.kstride), *vsrc = reinterpret_cast<const char*>(w.v + (tile0 + 1) * PA_TILE * w.vstride);
     auto ask = [&](int i, char* __restrict__ knew0, char* __restrict__ knew1, char* __restrict__ vnew0, char* __restrict__ vnew1) {
         if (i + 5 < tiles) {
-            asm volatile("" : "+v"(koff), "+v"(voff));  // (32-bit offsets to the scalar bases, not 64-bit addresses kept in registers)
+            const __amdgpu_buffer_rsrc_t kr = rows_at(ksrc), vr = rows_at(vsrc);
 #pragma unroll
             for (int k = 0; k < LOADS; ++k) {
-                __builtin_amdgcn_global_load_lds((const void*)(ksrc + k * krows + koff), (lds_ptr)(knew0 + (k * NW + wave) * 1024), 16, 0, 0);
-                __builtin_amdgcn_global_load_lds((const void*)(ksrc + (k + LOADS) * krows + koff), (lds_ptr)(knew1 + (k * NW + wave) * 1024), 16, 0, 0);
-                __builtin_amdgcn_global_load_lds((const void*)(vsrc + k * vrows + voff), (lds_ptr)(vnew0 + (k * NW + wave) * 1024), 16, 0, 0);
-                __builtin_amdgcn_global_load_lds((const void*)(vsrc + (k + LOADS) * vrows + voff), (lds_ptr)(vnew1 + (k * NW + wave) * 1024), 16, 0, 0);
+                dma(kr, knew0 + (k * NW + wave) * 1024, koff, k * krows);
+                dma(kr, knew1 + (k * NW + wave) * 1024, koff, (k + LOADS) * krows);
+                dma(vr, vnew0 + (k * NW + wave) * 1024, voff, k * vrows);
+                dma(vr, vnew1 + (k * NW + wave) * 1024, voff, (k + LOADS) * vrows);
             }
-            ksrc += 2 * LOADS * krows;
-            vsrc += 2 * LOADS * vrows;
+            ksrc += 2l * LOADS * krows;
+            vsrc += 2l * LOADS * vrows;
         } else {
             fetch(w.k, w.kstride, i + 3, knew0);
             fetch(w.k, w.kstride, i + 4, knew1);
