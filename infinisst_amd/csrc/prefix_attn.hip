@@ -326,9 +326,20 @@ __device__ __forceinline__ void block_role(const isst_prefix_attn& a, const Pref
         }
         if (i & 1) turn();
         ++i;
-        if (!(i & 1))
-            for (; i + 1 < whole; i += 2)
-                two_steps(i, kring + stage(i + 3), kring + stage(i), vring + stage(i + 1), vring + stage(i + 2), kring + stage(i + 1), kring + stage(i + 2), vring + stage(i + 3), vring + stage(i));
+        if (!(i & 1)) {
+            auto at = [&](int i, int r) {  // r = i mod 4
+                two_steps(i, kring + stage(r + 3), kring + stage(r), vring + stage(r + 1), vring + stage(r + 2), kring + stage(r + 1), kring + stage(r + 2), vring + stage(r + 3), vring + stage(r));
+            };
+            while (i + 1 < whole) {
+                if (i & 2) {
+                    at(i, 2);
+                    i += 2;
+                    if (i + 1 >= whole) break;
+                }
+                at(i, 0);
+                i += 2;
+            }
+        }
     }
     if (before != NONE) add_values(mine - 1);
     __syncthreads();  // (the last values are read behind the last turn)
