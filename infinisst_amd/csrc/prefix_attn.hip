@@ -10,7 +10,7 @@
 // O^T = V^T P^T wants its B operand in (the order of the keys inside a 16- or 32-key step is free as long as V^T is read in the same order: two transposed LDS reads).
 // The weights enter the value product as bf16 (2^-9 relative each, against the 2^-9 of the output's own rounding) and their sum is taken of the rounded ones, so that they still add up to
 // one; scores, references, sums and accumulators are fp32.
-// Measured, 32 heads over 8 key heads of 128: 64 sequences x 16 rows over 8192 shared keys 151 us = 910 TFLOP/s (a large matrix product of the library reaches 1192 on the same card);
+// Measured, 32 heads over 8 key heads of 128: 64 sequences x 16 rows over 8192 shared keys 157 us, the first launch 142 = 968 TFLOP/s (a large matrix product of the library reaches 1192 on the same card);
 // 64 x 1 row over 1000 own keys 47 us = 5.5 TB/s (a large copy: 4.9, counted both ways).
 #include "../../include/infinisst_hip.h"
 #include "common.h"
@@ -105,9 +105,10 @@ __device__ void add_keys(const isst_prefix_attn& a, const PrefixPlan& p, const K
 
 // ---------------------------------------------------------------------------------------------------------------- block role
 // columns [c0, c0 + 32 NW) against the key tiles of span `split` of `splits`.  A wave owns 32 columns.  Key and value tiles arrive by LDS-DMA in rings of four stages (64 KB: two workgroups a
-// CU), two tiles between barriers.  The matrix instructions of a tile are 512 cycles of the matrix pipe, its vector instructions 440 cycles of issue: one after the other the two waves of a
-// SIMD reached 750 TFLOP/s (tiles through registers, one a barrier), the same with LDS-DMA; exponentials between the matrix instructions of the neighbouring tiles 840; two tiles a barrier and
-// no 64-bit address arithmetic per tile 910, with the matrix pipe busy half of the time.
+// CU), two tiles between barriers.  The matrix instructions of a tile are 512 cycles of the matrix pipe, its vector instructions 315 cycles of issue: one after the other the two waves of a
+// SIMD take 184 us for 64 x 16 rows over 8192 keys, join included (tiles through registers or by LDS-DMA, one a barrier); with the exponentials between the matrix instructions of the neighbouring
+// tiles 176; two tiles a barrier and no 64-bit address arithmetic per tile 166; fragment waits counted 160; the ring's stages as constants 157.  The matrix pipe is then busy 56 % of the time
+// that a workgroup runs, at 1.98 GHz; the waves wait for it or for each other's.
 template <int D, int NW>
 __device__ __forceinline__ void block_role(const isst_prefix_attn& a, const PrefixPlan& p, char* lds, const KeySpan& w, int c0, int split, int splits, int slot) {
     constexpr int ROWB = 2 * D, CH = D / 8, LOADS = PA_TILE * CH / (NW * 64), RSTEP = NW * 64 / CH, QS = D / 16, DT = D / 32, STAGE = PA_TILE * ROWB;
