@@ -24,7 +24,8 @@ typedef __attribute__((address_space(3))) void* lds_ptr;
 
 #define PA_NW 4                  // waves of a workgroup, two workgroups a CU: the waits of one hide behind the other (eight waves, one a CU: 64 x 16 rows 151 -> 158 us, 64 x 5 rows 78 -> 92)
 #define PA_TILE 32               // keys of a block tile
-#define PA_RAISE 0x1p16f         // sum of a lane's weights in a step from which a column's reference is raised
+#define PA_HEAD 16.f             // octaves by which a column's reference stands above the maximum that set it
+#define PA_RAISE 1.f             // sum of a lane's weights in a step from which a column's reference is raised
 
 // [first, first + n) = the rows of sequence b, clipped to the launch's rows
 __device__ __forceinline__ void seq_rows(const isst_prefix_attn& a, int b, int& first, int& n) {
@@ -53,7 +54,7 @@ struct PrefixPlan {
     int own_block, own_tiles, own_splits, own_units;                           // column tiles of a sequence (a longer one walks on), key spans
     int slots;
     float* o;                                    // [slots][rows * heads][D] fp32, unnormalised
-    float2* ml;                                  // [slots][rows * heads]: maximum (in units of log2), sum
+    float2* ml;                                  // [slots][rows * heads]: reference (in units of log2), sum
 };
 // x / G for a column counted from the start of a row (x < G + 128, G < 2^15: exact)
 __device__ __forceinline__ int group_of(int x, unsigned magic) { return magic ? (int)__umulhi((unsigned)x, magic) : x; }
@@ -179,12 +180,12 @@ __device__ __forceinline__ void block_role(const isst_prefix_attn& a, const Pref
     };
     f32x16_t sc = scores(kring);  // (no tile: of whatever the stage holds, unused -- as behind the last tile below)
     turn();                       // (keys 4 take the place of keys 0)
-    // m becomes the maximum of what it covers and of these scores
+    // m becomes the maximum of what it covers and of these scores, and PA_HEAD
     auto raise = [&]() {
         float mx = sc[0];
 #pragma unroll
         for (int r = 1; r < 16; ++r) mx = fmaxf(mx, sc[r]);
-        mx = fmaxf(mx, __shfl_xor(mx, 32, WAVE)) * c2;
+        mx = __builtin_fmaf(fmaxf(mx, __shfl_xor(mx, 32, WAVE)), c2, PA_HEAD);
         const float m2 = fmaxf(m, mx), keep = m == m2 ? 1.f : m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - m2);
         l *= keep;
 #pragma unroll
@@ -209,9 +210,10 @@ __device__ __forceinline__ void block_role(const isst_prefix_attn& a, const Pref
         return sum;
     };
     // Step i: the scores of tile i are in sc and become weights; on the way the values of tile i - 1, whose weights are in pf, are added and the scores of tile i + 1 are computed.
-    // A column's reference m is the maximum of its first tile (and of its edge tiles): weights are exponentials against it, bf16 and fp32 hold them to 2^127, and no bit is lost by their
-    // size.  So other maxima are not looked for -- that and the running sum were 100 of the 169 vector instructions of a tile -- and only weights that pass PA_RAISE (or NaN) move m,
-    // before anything of the tile was used.  (2^16, so that values up to 2^90 cannot overflow the accumulators; scores have to rise by 11 above a column's first tile to get there.)
+    // A column's reference m stands 16 octaves above the maximum of its first tile (and of its edge tiles): weights are exponentials against it, bf16 and fp32 lose no bit by their size, so other
+    // maxima are not looked for -- that and the running sum were 100 of the 169 vector instructions of a tile -- and only weights whose sum in a lane passes one (or is NaN) move m, before
+    // anything of the tile was used.  A weight that is used is at most one, as with a running maximum: the accumulators hold whatever sum |v| over the keys does.  Scores have to rise by 11
+    // above a column's first tile to move m.  (A reference at the maximum itself and weights up to 2^16 took the same time, and values above 2^111 overflowed.)
     u32x4_t pf[2];
     enum { NONE, WHOLE, EDGE } before = NONE;  // what tile i - 1 was: EDGE, some column did not see some key of it
     auto ref = [&]() { return m == -INFINITY ? 0.f : -m; };
@@ -462,7 +464,7 @@ __device__ __forceinline__ void span_role(const isst_prefix_attn& a, const Prefi
                 for (int s = 0; s < QS; ++s) sc[n][t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf[t][s], __builtin_bit_cast(bf16x8_t, qf[n][s]), sc[n][t], 0, 0, 0);
             }
         const bool edge = j0 + 32 > see_least;  // some column does not see some key of this step
-        auto raise = [&]() {  // m becomes the maximum of what it covers and of these scores
+        auto raise = [&]() {  // m becomes the maximum of what it covers and of these scores, and PA_HEAD
 #pragma unroll
             for (int n = 0; n < NQ; ++n) {
                 float mx = sc[n][0][0];
@@ -471,7 +473,7 @@ __device__ __forceinline__ void span_role(const isst_prefix_attn& a, const Prefi
 #pragma unroll
                     for (int r = 0; r < 4; ++r) mx = fmaxf(mx, sc[n][t][r]);
                 mx = fmaxf(mx, __shfl_xor(mx, 16, WAVE));
-                mx = fmaxf(mx, __shfl_xor(mx, 32, WAVE)) * c2;
+                mx = __builtin_fmaf(fmaxf(mx, __shfl_xor(mx, 32, WAVE)), c2, PA_HEAD);
                 const float m2 = fmaxf(m[n], mx), keep = m[n] == m2 ? 1.f : m[n] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m[n] - m2);
                 l[n] *= keep;
 #pragma unroll

@@ -321,6 +321,19 @@ def test_prefix_attention_values_of_any_size():
         assert bool(((got - o).abs() <= U_BF * o.abs() + (U_BF + 2.0 ** -11) * A).all())  # (scores up to 34, not 20: 2^-12 becomes 2^-11)
 
 
+@pytest.mark.parametrize("rows,lens,P", [([3, 30], [90, 60], 3000), ([1, 2], [40, 9], 6500)])
+def test_prefix_attention_values_near_the_end_of_the_range(rows, lens, P):
+    """Positive values up to 2^118 behind scores that rise by eight (eleven octaves) inside a span, too little for a new reference: the outputs end below 2^119, and no accumulator may pass 2^128."""
+    q, kp, vp, kt, vt, ln, st = attn_inputs(35, rows, lens, 4, 2, 128, P, 96)
+    at = torch.arange(P, device=DEV)
+    q[..., 0], kt[..., 0] = 8.0, 0.0
+    kp[..., 0] = torch.where((at // 32 % 4 > 1) if max(rows) > 8 else (at >= 3072), 11.0, 0.0).to(BF)  # (two tiles low, two high; or every step of a wave but its first)
+    vp2, vt2 = vp.abs() * 2.0 ** 116, vt.abs() * 2.0 ** 116
+    o, A = attn_ref(q, kp, vp2, kt, vt2, ln, st)
+    got = E.op_prefix_attention(q, kp, vp2, kt, vt2, ln, st, max(rows)).cpu().double()
+    assert bool(((got - o).abs() <= U_BF * o.abs() + (U_BF + 2.0 ** -11) * A).all())  # (scores up to 34, not 20: 2^-12 becomes 2^-11)
+
+
 # ---------------------------------------------------------------------------------------------------------------- adapters
 def lora_inputs(seed, M, N, K, rank, n, ids):
     g = torch.Generator().manual_seed(seed)
