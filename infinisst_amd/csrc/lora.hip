@@ -138,7 +138,7 @@ __global__ __launch_bounds__(LORA_DOWN_WAVES * 64) void lora_down_kernel(LoraArg
     }
 }
 
-// Units: row tile fastest, then column tile of 64 CG.  t enters the product as a pair of bf16 numbers (hi, lo: 2^-16 relative) side by side along the product's depth, both against the same entries
+// Units: row tile fastest, then column tile of 64 CG.  t enters the product as a pair of bf16 numbers (hi, lo: 2^-15 relative) side by side along the product's depth, both against the same entries
 // of up.  CG = 1: the waves take an adapter each (few workgroups: decode steps; 64 rows with 64 adapters 6.9 us, with CG = 4 13.5); CG = 4: a column group each
 // (t is summed once for 256 columns: 1408 rows 19 us, with CG = 1 26).  Bound by the base's fp32 slices: 46 MB at 1408 rows, 42 MB at 320
 template <int RT, int CG>
@@ -202,13 +202,16 @@ __global__ __launch_bounds__(256) void lora_up_kernel(LoraArgs g, int tiles, int
                 }
                 v *= scale;
             }
-            f32x4_t lo;
+            // hi = the bf16 number below |v| and never v itself, so that lo has v's sign and is zero only where v is: an infinite entry of up times the pair is then up times v, and no v below
+            // fp32's end rounds to infinity (v infinite: hi finite, lo infinite)
+            f32x4_t hi, lo;
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
-                const float hi = bfr(v[k]);
-                lo[k] = __builtin_isfinite(hi) ? v[k] - hi : 0.f;
+                const unsigned bits = __float_as_uint(v[k]);
+                hi[k] = __uint_as_float((bits - ((bits & 0x7fffffffu) != 0u)) & 0xffff0000u);
+                lo[k] = v[k] - hi[k];
             }
-            *reinterpret_cast<u32x2_t*>(&th[0][row][r]) = (u32x2_t){pack_bf(v.x, v.y), pack_bf(v.z, v.w)};
+            *reinterpret_cast<u32x2_t*>(&th[0][row][r]) = (u32x2_t){pack_bf(hi.x, hi.y), pack_bf(hi.z, hi.w)};
             *reinterpret_cast<u32x2_t*>(&th[1][row][r]) = (u32x2_t){pack_bf(lo.x, lo.y), pack_bf(lo.z, lo.w)};
         }
         __syncthreads();

@@ -410,6 +410,32 @@ def test_gemm_lora_adapters_do_not_mix():
     assert not bool(torch.isfinite(got[hit][:, 5]).any()) and torch.equal(got[hit][:, 6:], clean[hit][:, 6:])
 
 
+@pytest.mark.parametrize("M,N", [(40, 96), (1040, 1031)])
+def test_gemm_lora_infinite_entries_have_the_sign_of_the_formula(M, N):
+    """An infinite entry of `up` times an inner product that a bf16 number holds exactly, and one that it does not; zero times infinity is NaN; an inner product just below the end of fp32 stays finite."""
+    K, rank = 256, 16
+    g = torch.Generator().manual_seed(5)
+    x, W = torch.zeros(M, K, dtype=BF), torch.zeros(N, K, dtype=BF)
+    x[:, 0], x[:, 1] = torch.tensor([1.0, -2.0, 0.75, -96.0]).repeat(M)[:M].to(BF), torch.tensor([0.5, 0.0, -3.0]).repeat(M)[:M].to(BF)
+    x[:, 2:60] = torch.randn(M, 58, generator=g).to(BF)
+    x[:, 100], x[:, 101] = 3.3895313892515355e38, 2.0 ** 119
+    down, up = torch.zeros(2, rank, K, dtype=BF), torch.zeros(2, N, rank, dtype=BF)
+    down[1, 3, 0] = down[1, 0, 1] = down[1, 9, 100] = down[1, 9, 101] = 1.0
+    down[1, 7, 2:60] = 0.25
+    up[1, 5, 3], up[1, 9, 0], up[1, 13, 7], up[1, 17, 9] = math.inf, -math.inf, math.inf, 2.0 ** -90
+    ids = torch.arange(M, dtype=torch.int32) % 3
+    got = lora_run(x, W, down, up, torch.tensor([1.0, 1.0]), ids).double().cpu()
+    rows = ids == 1
+    xd = x.double()[rows]
+    inner = xd[:, 2:60].sum(1)
+    want = torch.zeros(int(rows.sum()), N, dtype=torch.float64)
+    want[:, 5], want[:, 9], want[:, 13] = xd[:, 0] * math.inf, xd[:, 1] * -math.inf, inner * math.inf
+    want[:, 17] = (xd[:, 100] + xd[:, 101]) * 2.0 ** -90  # (half way between the largest bf16 number and infinity)
+    assert bool((got[~rows] == 0.0).all())
+    ok = (got[rows] == want) | (torch.isnan(got[rows]) & torch.isnan(want)) | ((got[rows] - want).abs() <= U_BF * want.abs() + 2 * U_BF ** 2 * want.abs())
+    assert bool(ok.all()), (~ok).nonzero()[:5]
+
+
 def test_gemm_lora_strided():
     M, N, K, rank, n = 30, 144, 512, 16, 3
     x, W, down, up, scales, ids = lora_inputs(2, M, N, K, rank, n, [m % 4 - 1 for m in range(M)])
