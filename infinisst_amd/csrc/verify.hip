@@ -20,15 +20,15 @@ struct VerifyStat { double sum; float max; int at; };  // of a slice: sum of exp
 
 typedef float f32x4u_t __attribute__((ext_vector_type(4), aligned(4)));  // (rows start anywhere)
 
-// exp(d) for -700 <= d <= 0: 2^k exp(r), k the nearest whole number to d / ln 2 (added to 1.5 2^52, where it is the low word), |r| <= ln 2 / 2, the polynomial of degree 8 through exp at the
-// Chebyshev nodes of that interval.  Its error is below 1.1e-12 relative (checked against 60 digits on 4001 points): over 128 k borders of an inverse CDF one draw in 10^7 could land elsewhere
-// for it.  The score read is bound by these instructions -- a 64-bit multiply-add an entry is 2.4 us of the 82 that 64 streams x 4 drafts with scores take (Taylor to r^10 / 10!, 2.2e-13: 86 us;
-// degree 9, 2e-14: 84).
+// exp(d) for -700 <= d <= 0: 2^k exp(r), k the nearest whole number to d / ln 2 (added to 1.5 2^52, where it is the low word), |r| <= ln 2 / 2, the polynomial of degree 10 through exp at the
+// Chebyshev nodes of that interval.  Relative error (checked against 60 digits on 4001 points): 4.3e-16 of the polynomial, i.e. two roundings, and 2.4e-17 |k| of the one-term reduction -- 1.7e-15
+// down to d = -40; over 128 k borders of an inverse CDF one draw in 10^9 could land elsewhere for it.  The score read is bound by these instructions, a 64-bit multiply-add an entry is 2.4 us of the
+// 84 that 64 streams x 4 drafts with scores take (degree 8, 1.05e-12: 80 -- but then uniforms 1e-12 beside a probability are decided wrongly).
 __device__ __forceinline__ double exp_core(double d) {
     const double t = fma(d, 1.4426950408889634074, 0x1.8p52), k = t - 0x1.8p52, r = fma(-k, 0.69314718055994530942, d);
-    double p = 2.487616403756168e-05;
-    p = fma(p, r, 0.00019915866941726544); p = fma(p, r, 0.0013888821677603455); p = fma(p, r, 0.008333266097922691); p = fma(p, r, 0.04166666689095713);
-    p = fma(p, r, 0.16666666891045911); p = fma(p, r, 0.49999999999797934); p = fma(p, r, 0.9999999999797852); p = fma(p, r, 1.0);
+    double p = 2.7626426376580335e-07;
+    p = fma(p, r, 2.7640263790318923e-06); p = fma(p, r, 2.4801504180837137e-05); p = fma(p, r, 0.00019841170070971308); p = fma(p, r, 0.0013888888932619635); p = fma(p, r, 0.008333333385825085);
+    p = fma(p, r, 0.04166666666657277); p = fma(p, r, 0.16666666666553953); p = fma(p, r, 0.5000000000000006); p = fma(p, r, 1.0000000000000069); p = fma(p, r, 1.0);
     return __hiloint2double(__double2hiint(p) + (__double2loint(t) << 20), __double2loint(p));
 }
 // ... for any d <= 0; under -700 and for NaN (-inf less -inf): 0

@@ -597,6 +597,26 @@ def test_verify_drafts_rows_behind_the_drafts_do_not_matter():
         verify_same((t, drafts, n, q if kind == "scores" else None, None if kind == "greedy" else u))
 
 
+@pytest.mark.parametrize("B,V", [(64, 50), (16, 5000)])
+def test_verify_drafts_compare_in_64_bits(B, V):
+    """A draft without scores is accepted at a uniform 2^-46 (relative) below its probability and refused 2^-46 above it.  The probability's own error is below half of that: an exponential 1.3e-15
+    (its polynomial 4.3e-16, the reduced argument 2.4e-17 |k| with |k| <= 36), up to 40 additions and products of a sum 4.5e-15, 1.3e-15 for its terms, the quotient 1.1e-16."""
+    from decimal import Decimal, localcontext
+    rng = np.random.default_rng(V)
+    t = (rng.standard_normal((B, 2, V)) * 2.0).astype(np.float32)
+    drafts = rng.integers(0, V, (B, 1)).astype(np.int32)
+    drafts[: B // 2, 0] = t[: B // 2, 0].argmax(-1)
+    p = []
+    with localcontext() as ctx:
+        ctx.prec = 40
+        for b in range(B):
+            e = [(Decimal(float(s)) - Decimal(float(t[b, 0].max()))).exp() for s in t[b, 0]]
+            p.append(e[drafts[b, 0]] / sum(e))
+        u = np.array([[[float(pb * (1 + side * Decimal(2) ** -46)), 0.5] for pb in p] for side in (-1, 1)])
+    below, above = verify_run(t, drafts, None, None, u[0])[1], verify_run(t, drafts, None, None, u[1])[1]
+    assert (below == 2).all() and (above == 1).all(), (int((below != 2).sum()), int((above != 1).sum()))
+
+
 def test_verify_drafts_strided_scores():
     t, drafts, n, q, u = verify_inputs(10, 3, 2, 1031)
     wide = torch.zeros(3, 4, 1100, device=DEV)
