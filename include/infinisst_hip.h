@@ -293,7 +293,7 @@ int isst_op_gemm_attn_merge(const float* partial, int n_splits, const uint16_t* 
  * softmax(q k^T) v, keys already rotated).  Sequence b owns rows row_starts[b] .. row_starts[b + 1] - 1 (NULL: rows / seqs each) = its newest positions: row t of n
  * sees every prefix key and the own keys 0 .. tail_lens[b] - n + t.  A row that sees no key gives zeros; rows outside every sequence are left as they were.
  * Strides in elements (multiples of 8, a key's 0 .. 2^24), every row of head_dim elements contiguous and 16-byte aligned; rows * heads <= 2^26, heads <= 2^15,
- * seqs * kv_heads <= 2^22.  tail_lens is read as clamped to 0 .. tail_cap, row_starts (non-decreasing)
+ * seqs * kv_heads <= 2^22.  out keeps the heads of a row together or the rows of a head, without overlap (it may be q).  tail_lens is read as clamped to 0 .. tail_cap, row_starts (non-decreasing)
  * to 0 .. rows: nothing outside the arrays is touched whatever they hold. */
 typedef struct isst_prefix_attn {
     const uint16_t* q;              /* [rows][heads][head_dim] */

@@ -275,8 +275,10 @@ static bool prefix_attention_ok(const isst_prefix_attn* a) {
     if (strides & 7) return false;
     for (const int64_t key : {a->kp_key, a->vp_key, a->kt_key, a->vt_key})  // (32-bit offsets inside a tile of 32 keys)
         if (key < 0 || key > (1 << 24)) return false;
-    // two outputs never share memory
-    return (a->heads == 1 || a->out_head >= a->head_dim) && (a->rows == 1 || a->out_row >= (a->heads - 1) * a->out_head + a->head_dim);
+    // two outputs never share memory: the heads of a row lie together, or the rows of a head
+    const bool one_head = a->heads == 1, one_row = a->rows == 1;
+    if ((!one_head && a->out_head < a->head_dim) || (!one_row && a->out_row < a->head_dim)) return false;
+    return one_head || one_row || (a->out_row - a->head_dim) / a->out_head >= a->heads - 1 || (a->out_head - a->head_dim) / a->out_row >= a->rows - 1;
 }
 extern "C" int64_t isst_op_prefix_attention_workspace(const isst_prefix_attn* a) { return prefix_attention_ok(a) ? (a->rows ? prefix_attention_workspace(*a) : 0) : ISST_ERR_ARG; }
 extern "C" int isst_op_prefix_attention(const isst_prefix_attn* a, void* workspace, int64_t workspace_bytes, void* hip_stream) {

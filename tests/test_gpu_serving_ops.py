@@ -277,6 +277,16 @@ def test_prefix_attention_in_place_and_one_key_for_all():
     attn_check(E.op_prefix_attention(q, one_k, one_v, kt, vt, ln, st, 40), o, A)
 
 
+def test_prefix_attention_head_major_output():
+    """The output as a view of [heads][rows]: the same values, and nothing around them."""
+    q, kp, vp, kt, vt, ln, st = attn_inputs(51, [2, 40], [9, 50], 8, 2, 128, 90, 64)
+    want = E.op_prefix_attention(q, kp, vp, kt, vt, ln, st, 40)
+    whole = torch.full((8, 42, 144), 7.0, dtype=BF, device=DEV)
+    out = whole[:, :, 8:136].transpose(0, 1)
+    E.op_prefix_attention(q, kp, vp, kt, vt, ln, st, 40, out=out)
+    assert torch.equal(out, want) and bool((whole[:, :, :8] == 7.0).all()) and bool((whole[:, :, 136:] == 7.0).all())
+
+
 @pytest.mark.parametrize("R,L,P,H,KV,D", [(1500, 1500, 0, 4, 2, 128), (1100, 2300, 77, 3, 3, 64)])
 def test_prefix_attention_whole_prompt_of_one_sequence(R, L, P, H, KV, D):
     """A prompt pass: every row of a long sequence at once, causal over its own keys, beside a sequence of one row."""

@@ -45,6 +45,15 @@ def test_prefix_attention_size_limits(lib):
         assert ws(**{key: 1 << 24}) > 0 and ws(**{key: (1 << 24) + 8}) == -1 and ws(**{key: -8}) == -1
 
 
+def test_prefix_attention_output_orders(lib):
+    """Outputs of a row together or of a head together, never overlapping (3 rows, 4 heads of 128)."""
+    ws = lambda row, head, **kw: lib.isst_op_prefix_attention_workspace(C.byref(attn(out_row=row, out_head=head, **kw)))
+    assert ws(512, 128) > 0 and ws(128, 384) > 0 and ws(136, 400) > 0 and ws(1 << 40, 1 << 20) > 0 and ws(1 << 20, 1 << 40) > 0
+    for row, head in ((504, 128), (128, 376), (120, 400), (512, 120), (128, 128), (0, 384), (-128, 512), (512, -128)):
+        assert ws(row, head) == -1, (row, head)
+    assert ws(0, 128, rows=1, seqs=1) > 0 and ws(128, 0, heads=1, kv_heads=1) > 0
+
+
 def test_prefix_attention_workspace(lib):
     assert lib.isst_op_prefix_attention(None, None, 0, None) == -1 and lib.isst_op_prefix_attention_workspace(None) == -1
     a = attn()
