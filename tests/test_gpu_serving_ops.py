@@ -171,6 +171,26 @@ def test_prefix_attention_masked_values_do_not_reach_a_row():
     attn_check(got[7][:, keep], o[7][:, keep], A[7][:, keep])
 
 
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("H,KV", [(4, 1), (2, 2)])
+def test_prefix_attention_masked_values_among_many_columns(H, KV, D):
+    """As above where a workgroup takes 128 columns: infinite and NaN values in neighbouring tiles that only the newest rows see, and in the last, partial tile of the prefix."""
+    rows, lens, P, cap = [40, 70, 33], [100, 150, 33], 45, 160
+    q, kp, vp, kt, vt, ln, st = attn_inputs(10, rows, lens, H, KV, D, P, cap)
+    vt[0, 0, 95, 3], vt[0, 0, 97, 5], kt[0, 0, 99] = math.inf, math.nan, math.nan  # row t of sequence 0 sees the keys up to 60 + t
+    vt[1, KV - 1, 120, 7], vt[1, :, 149], vt[1, 0, 127, 9], vt[1, 0, 128, 9] = math.nan, -math.inf, math.inf, math.inf  # ... of sequence 1 up to 80 + t
+    vt[2, :, 1, 2], vt[2, :, 32, 60] = -math.inf, math.inf  # ... of sequence 2 up to t
+    vp[0, 40, 11], vp[KV - 1, 44, 13] = math.inf, -math.inf
+    o, A = attn_ref(q, kp, vp, kt, vt, ln, st)
+    got = E.op_prefix_attention(q, kp, vp, kt, vt, ln, st, 70).cpu().double()
+    same = (torch.isnan(got) & torch.isnan(o)) | (got == o)
+    fine = torch.isfinite(o)
+    assert bool(same[~fine].all()), (~same & ~fine).nonzero()[:5]
+    assert 0.5 < float(fine.double().mean()) < 1.0
+    tol = U_BF * o.abs() + (U_BF + 2.0 ** -12) * A
+    assert bool(((got - o).abs() <= tol)[fine].all()), (~((got - o).abs() <= tol) & fine).nonzero()[:5]
+
+
 def test_prefix_attention_large_scores():
     """Scores in the thousands (one key takes everything) and scores that differ by less than a rounding."""
     q, kp, vp, kt, vt, ln, st = attn_inputs(11, [2, 2], [10, 70], 4, 2, 128, 100, 80)
