@@ -413,6 +413,18 @@ def test_gemm_lora_row_orders(M, N, K, rank, n, spread):
     lora_check(lora_run(*args), *args, what=spread)
 
 
+@pytest.mark.parametrize("M,N,K,rank", [(65, 2064, 4096, 16), (65, 2051, 4096, 16), (130, 2064, 4096, 32), (130, 2051, 4096, 16), (256, 2064, 4096, 64), (256, 2051, 4096, 16), (130, 600, 14336, 40)])
+def test_gemm_lora_long_weights(M, N, K, rank):
+    """65 to 256 rows of a weight of eight million entries and more (13 to 51 streams of five rows through a full-size projection): a base kernel of its own, whole and ragged columns."""
+    n = 7
+    rng = np.random.default_rng(M + N)
+    args = lora_inputs(M + rank, M, N, K, rank, n, rng.integers(-1, n, M).tolist())
+    print(M, N, K, rank, flush=True)
+    got = lora_run(*args)
+    lora_check(got, *args, what=f"M{M} N{N} K{K} r{rank}")
+    assert torch.equal(got, lora_run(*args))
+
+
 @pytest.mark.parametrize("rank", [8, 16, 24, 32, 40, 64, 72, 96, 128])
 def test_gemm_lora_many_rows_of_every_rank(rank):
     """Enough rows and columns for the wide form of the adapter sum (1040 x 1031: 65 x 17 tiles), runs of rows and a changing adapter per row, a column tail, K past one slice."""
@@ -475,6 +487,17 @@ def test_gemm_lora_strided():
     ref = lora_run(x, W, down, up, scales, ids)
     got = E.op_gemm_lora(wide[:, K:2 * K], E.op_pack_weight(W.to(DEV)), N, down.to(DEV), up.to(DEV), scales.to(DEV), ids.to(DEV), out=out[:, 8:8 + N])
     assert torch.equal(got, ref) and bool((out[:, :8] == 5.0).all()) and bool((out[:, 8 + N:] == 5.0).all())
+
+
+def test_gemm_lora_millions_of_rows():
+    """More rows than 65535 workgroups of the kernel without K slices take (64 rows each), at the smallest depth and width; 1009 rows repeated."""
+    M, N, K, rank, n, period = 64 * 65535 + 77, 16, 32, 8, 3, 1009
+    x, W, down, up, scales, ids = lora_inputs(7, period, N, K, rank, n, [m % 4 - 1 for m in range(period)])
+    many = torch.arange(M, device=DEV) % period
+    got = E.op_gemm_lora(x.to(DEV)[many], E.op_pack_weight(W.to(DEV)), N, down.to(DEV), up.to(DEV), scales.to(DEV), ids.to(DEV)[many])
+    first = got[:period]
+    lora_check(first, x, W, down, up, scales, ids)
+    assert torch.equal(got, first[many])  # (a row's sums do not depend on where it stands)
 
 
 def test_gemm_lora_in_place():
