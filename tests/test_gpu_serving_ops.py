@@ -590,6 +590,49 @@ def test_verify_drafts(B, K, V, kind):
         verify_same((t, drafts, None if seed == 2 else n, q if kind == "scores" and K else None, None if kind == "greedy" else u))
 
 
+def long_drafts(seed, B, K, V, stops, kind):
+    """Inputs whose stream b accepts stops[b][1] of stops[b][0] drafts: target and draft agree on the drafted token but at the refusal."""
+    t, drafts, n, q, u = verify_inputs(seed, B, K, V)
+    at = np.arange(K)
+    for b, (live, accepted) in enumerate(stops):
+        n[b] = live
+        t[b, at, drafts[b]] += 30.0
+        q[b, at, drafts[b]] += 28.0
+        if accepted < live:
+            t[b, accepted, drafts[b, accepted]] -= 60.0
+    return t, drafts, n, q if kind == "scores" else None, None if kind == "greedy" else u
+
+
+@pytest.mark.parametrize("kind", ["scores", "bare", "greedy"])
+def test_verify_drafts_more_than_32(kind):
+    K = 70
+    stops = [(70, a) for a in (0, 1, 31, 32, 33, 63, 64, 65, 69, 70)] + [(n, n) for n in (0, 31, 32, 33, 64, 65)] + [(33, 32), (65, 64), (32, 31)]
+    args = long_drafts(3, len(stops), K, 300, stops, kind)
+    assert verify_ref(*args)[1].tolist() == [a + 1 for _, a in stops]
+    verify_same(args)
+
+
+@pytest.mark.parametrize("V", [131073, 151936, 262145, 300001])
+@pytest.mark.parametrize("kind", ["scores", "bare", "greedy"])
+def test_verify_drafts_large_vocabularies(V, kind):
+    """More than 32 and more than 64 slices of 4096 scores; draws at both ends and past slice 64, drafts in the last slice, whole slices of removed entries."""
+    B, K = 6, 2
+    t, drafts, n, q, u = verify_inputs(V, B, K, V)
+    n[:] = K
+    drafts[3:, 0] = V - 1 - np.arange(3)
+    u[:, K] = [0.0, 0.5, 0.93, 0.9999, 1.0 - 2.0 ** -53, 0.97]
+    u[:, 0] = np.where(np.arange(B) % 2, 0.999999, u[:, 0])  # (mostly refused)
+    t[2, :, 4096 * 3:4096 * 30] = -np.inf
+    t[5, :, :V - 40] = -np.inf
+    drafts[5] = V - 7
+    if kind == "greedy":
+        drafts[:] = t[:, :K].argmax(-1)
+        drafts[1, 1] += -1 if drafts[1, 1] else 1
+        t[4, 1, V - 1] = t[4, 1, 5] = 60.0
+        drafts[4, 1] = 5
+    verify_same((t, drafts, n, q if kind == "scores" else None, None if kind == "greedy" else u))
+
+
 def test_verify_drafts_ties_and_removed_entries():
     """Greedy ties go to the lowest index; -inf entries are never drawn nor accepted; identical rows accept everything and their draw falls back to the row."""
     B, K, V = 6, 3, 5000
