@@ -336,7 +336,15 @@ extern "C" int isst_op_gemm_lora(const uint16_t* A, int64_t lda, const uint16_t*
     l.t = static_cast<float*>(workspace) + (int64_t)g.ksplit * M * g.N;
     l.out = out; l.ldo = ldo; l.M = M; l.N = N; l.K = K; l.rank = rank; l.n_adapters = n_adapters;
     int rc = launch_lora_down(l, st);
-    if (rc == ISST_OK) rc = launch_gemm(g, st);
+    // the kernel behind EPI_RAW has 64 rows a workgroup along the grid's second dimension, which ends at 65536 (depths that are no multiple of 64: M goes up to 2^24)
+    const int rows = g.epi == EPI_RAW ? 64 * 65535 : M;
+    for (int m0 = 0; rc == ISST_OK && m0 < M; m0 += rows) {
+        GemmArgs part = g;
+        part.A += (int64_t)m0 * lda;
+        part.out = static_cast<float*>(workspace) + (int64_t)m0 * g.N;
+        part.M = M - m0 < rows ? M - m0 : rows;
+        rc = launch_gemm(part, st);
+    }
     if (rc == ISST_OK) rc = launch_lora_up(l, st);
     return rc;
 }
