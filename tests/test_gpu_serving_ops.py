@@ -203,6 +203,20 @@ def test_prefix_attention_large_scores():
         assert bool(((got - o).abs() <= tol).all())
 
 
+@pytest.mark.parametrize("rows", [[1, 2], [40, 33]])
+@pytest.mark.parametrize("sign", [1.0, -1.0])
+def test_prefix_attention_scores_of_two_to_the_24(rows, sign):
+    """Scores of 2^24 and more, two apart, all of them exact in fp32 (8192 x 16384 + 16 n, times 1 / 8): their differences decide as between small scores."""
+    H, KV, D, P, cap = 4, 2, 64, 300, 160
+    q, kp, vp, kt, vt, ln, st = attn_inputs(25, rows, [r + 60 for r in rows], H, KV, D, P, cap)
+    q.zero_()
+    q[..., 0], q[..., 1] = 8192.0, 16.0
+    kp[..., 0], kt[..., 0] = sign * 16384.0, sign * 16384.0
+    kp[..., 1], kt[..., 1] = (torch.arange(P, device=DEV) * 7 % 5).to(BF), (torch.arange(cap, device=DEV) * 3 % 6).to(BF)
+    o, A = attn_ref(q, kp, vp, kt, vt, ln, st)
+    attn_check(E.op_prefix_attention(q, kp, vp, kt, vt, ln, st, max(rows)), o, A)
+
+
 @pytest.mark.parametrize("rows,D", [([1, 2], 128), ([40, 33], 128), ([1] * 40, 64)])
 @pytest.mark.parametrize("removed", [-math.inf, -3.3895313892515355e38])
 def test_prefix_attention_scores_of_minus_infinity(rows, D, removed):
