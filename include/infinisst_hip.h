@@ -293,8 +293,10 @@ int isst_op_gemm_attn_merge(const float* partial, int n_splits, const uint16_t* 
  * softmax(q k^T) v, keys already rotated).  Sequence b owns rows row_starts[b] .. row_starts[b + 1] - 1 (NULL: rows / seqs each) = its newest positions: row t of n
  * sees every prefix key and the own keys 0 .. tail_lens[b] - n + t.  A row that sees no key gives zeros; rows outside every sequence are left as they were.
  * Strides in elements (multiples of 8, a key's 0 .. 2^24), every row of head_dim elements contiguous and 16-byte aligned; rows * heads <= 2^26, heads <= 2^15,
- * seqs * kv_heads <= 2^22.  out keeps the heads of a row together or the rows of a head, without overlap (it may be q).  tail_lens is read as clamped to 0 .. tail_cap, row_starts (non-decreasing)
- * to 0 .. rows: nothing outside the arrays is touched whatever they hold. */
+ * seqs * kv_heads <= 2^22.  out keeps the heads of a row together or the rows of a head, without overlap (it may be q).  tail_lens is
+ * read as clamped to 0 .. tail_cap, row_starts (non-decreasing) to 0 .. rows: nothing outside the arrays is touched whatever they hold.
+ * Scores, sums and accumulators are fp32; softmax weights enter the value product rounded to bf16 and are summed so (2^-8 of a weight at most, on top of the output's own rounding).  Scores of any size
+ * up to 2^24 (scale * q.k; an fp32 score beyond has no fraction left to tell keys apart by), -inf included; values of any size as long as the |v| that a row sees add up to less than 2^128. */
 typedef struct isst_prefix_attn {
     const uint16_t* q;              /* [rows][heads][head_dim] */
     const uint16_t *k_prefix, *v_prefix; /* [kv_heads][prefix_len][head_dim] */
@@ -315,7 +317,7 @@ int isst_op_prefix_attention(const isst_prefix_attn* a, void* workspace, int64_t
 /* out[m] = bf16(A[m] W^T + scales[a] * (A[m] down[a]^T) up[a]^T), a = row_adapter[m]; a row whose a is outside 0 .. n_adapters - 1 has no adapter.  packed:
  * isst_op_pack_weight of W [N][K]; down [n_adapters][rank][K], up [n_adapters][N][rank] bf16 contiguous; rank a multiple of 8 up to 128; K % 32 == 0; M * K and M * lda
  * < 2^29, M * N < 2^30.
- * Sums stay in fp32, one rounding at the end.  F.linear next to per-request adapters; the reference has one set of weights per language pair instead. */
+ * Sums stay in fp32, one rounding at the end; infinite and NaN entries give what the formula gives, in the rows of their adapter only.  F.linear next to per-request adapters; the reference has one set of weights per language pair instead. */
 int64_t isst_op_gemm_lora_workspace(int M, int N, int K, int rank, int n_adapters);
 int isst_op_gemm_lora(const uint16_t* A, int64_t lda, const uint16_t* packed, const uint16_t* down, const uint16_t* up, const float* scales,
                       const int* row_adapter, int n_adapters, int rank, uint16_t* out, int64_t ldo, int M, int N, int K, void* workspace,

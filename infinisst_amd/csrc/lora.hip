@@ -4,8 +4,8 @@
 // Both kernels take tiles of 16 rows and walk the DISTINCT adapters of a tile: one matrix product per adapter for all 16 rows, of which every row keeps the one of its own adapter -- a
 // selection, so that another adapter's inf or NaN cannot reach it.  No sorting and no plan: neighbouring rows of a stream share an adapter (one or two products a tile), and a decode
 // step with an adapter per row reads each adapter once, as it has to.  Bound by the adapters' bytes and, below them, by latency.
-// Measured next to their base product (us, down + base + up; K x N, rank, rows): 4096 x 6144, 16, 1 row 4.0 + 8.8 + 4.0; 64 rows with 64 adapters 5.2 + 18 + 6.8; 14336 x 4096, 64, 320 rows
-// 12 + 49 + 14.3; 4096 x 4096, 32, 1408 rows 8.2 + 51 + 17.8.
+// Measured next to their base product (us, down + base + up; K x N, rank, rows): 4096 x 6144, 16, 1 row 3.9 + 8.7 + 3.9; 64 rows with 64 adapters 5.1 + 18 + 7.0; 14336 x 4096, 64, 320 rows
+// 12 + 48 + 14.3; 4096 x 4096, 32, 1408 rows 8.2 + 46 + 17.2.
 #include "common.h"
 #include "kernels.h"
 

@@ -8,10 +8,11 @@
 //   span:  16 NQ columns of ONE sequence against its own keys (or of the whole batch against the prefix where it has no more columns than that); the waves split the keys.  Bound by the read.
 // Scores are computed transposed, S^T = K Q^T, so that a lane holds one column: statistics and rescaling are per lane, and the exponentials are already in the layout the value product
 // O^T = V^T P^T wants its B operand in (the order of the keys inside a 16- or 32-key step is free as long as V^T is read in the same order: two transposed LDS reads).
-// The weights enter the value product as bf16 (2^-9 relative each, against the 2^-9 of the output's own rounding) and their sum is taken of the rounded ones, so that they still add up to
-// one; scores, references, sums and accumulators are fp32.
-// Measured, 32 heads over 8 key heads of 128: 64 sequences x 16 rows over 8192 shared keys 157 us, the first launch 142 = 968 TFLOP/s (a large matrix product of the library reaches 1192 on the same card);
-// 64 x 1 row over 1000 own keys 47 us = 5.5 TB/s (a large copy: 4.9, counted both ways).
+// The weights enter the value product as bf16 (off by 2^-8 relative at most, as the output's own rounding is) and their sum is taken of the rounded ones, so that they still add up to one: bf16
+// matrix instructions want both operands so, and a pair of bf16 numbers a weight would double that product.  Over a row's norm the outputs are off by 0.0020 to 0.0024, by 0.0017 from their own rounding
+// alone.  Scores, references, sums and accumulators are fp32.
+// Measured, 32 heads over 8 key heads of 128: 64 sequences x 16 rows over 8192 shared keys 143 us a call, the first launch 131 = 1048 TFLOP/s (a large matrix product of the library reaches 1192 on the
+// same card); 64 x 1 row over 1000 own keys 47 us = 5.5 TB/s (a large copy: 4.9, counted both ways).
 #include "../../include/infinisst_hip.h"
 #include "common.h"
 #include "kernels.h"
@@ -85,7 +86,7 @@ __device__ __forceinline__ void dma(const __amdgpu_buffer_rsrc_t& r, char* dst, 
     __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lds_ptr)dst, 16, lane_offset, rows_offset, 0, 0);
 }
 
-// Keys [lo, hi) of one column added to its stored partial result, whose maximum covers them.  Only for tiles that hold inf or NaN values and that some column of a wave does not see
+// Keys [lo, hi) of one column added to its stored partial result, whose reference covers them.  Only for tiles that hold inf or NaN values and that some column of a wave does not see
 // whole: in a matrix product 0 x inf would reach the columns that do not see the key.
 template <int D>
 __device__ void add_keys(const isst_prefix_attn& a, const PrefixPlan& p, const KeySpan& w, int slot, int c, int lo, int hi) {
@@ -108,8 +109,8 @@ __device__ void add_keys(const isst_prefix_attn& a, const PrefixPlan& p, const K
 // columns [c0, c0 + 32 NW) against the key tiles of span `split` of `splits`.  A wave owns 32 columns.  Key and value tiles arrive by LDS-DMA in rings of four stages (64 KB: two workgroups a
 // CU), two tiles between barriers.  The matrix instructions of a tile are 512 cycles of the matrix pipe, its vector instructions 315 cycles of issue: one after the other the two waves of a
 // SIMD take 184 us for 64 x 16 rows over 8192 keys, join included (tiles through registers or by LDS-DMA, one a barrier); with the exponentials between the matrix instructions of the neighbouring
-// tiles 176; two tiles a barrier and no 64-bit address arithmetic per tile 166; fragment waits counted 160; the ring's stages as constants 157.  The matrix pipe is then busy 56 % of the time
-// that a workgroup runs, at 1.98 GHz; the waves wait for it or for each other's.
+// tiles 176; two tiles a barrier and no 64-bit address arithmetic per tile 166; fragment waits counted 160; the ring's stages as constants 157.  (All of these on a chip that 20 calls
+// do not bring to its clock; in the long run the last form takes 143.)  The matrix pipe is busy 56 % of the time that a workgroup runs; the waves wait for it or for each other's.
 template <int D, int NW>
 __device__ __forceinline__ void block_role(const isst_prefix_attn& a, const PrefixPlan& p, char* lds, const KeySpan& w, int c0, int split, int splits, int slot) {
     constexpr int ROWB = 2 * D, CH = D / 8, LOADS = PA_TILE * CH / (NW * 64), RSTEP = NW * 64 / CH, QS = D / 16, DT = D / 32, STAGE = PA_TILE * ROWB;

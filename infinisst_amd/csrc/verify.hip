@@ -5,7 +5,7 @@
 // Launch 1 reads every score row once, a workgroup per slice of VF_SLICE entries (maximum and its first index, or sum of exponentials); its floor is that read, and most of
 // the 64-bit exponentials hides behind it.  Drafts with scores need two more: who decides (a workgroup per stream), and what a refused draft leaves over, slice by slice.  The last
 // launch takes one workgroup per stream: find the slice that the draw falls into from the slice sums, walk that slice.
-// Measured, rows of 128263: 64 streams x 4 drafts with scores 57 us (265 MB: 4.6 TB/s) + decide 4.8 + left over 14.3 + draw 6.8; one stream without scores 6.2 + 6.6, latency all of it (in cycles
+// Measured, rows of 128263: 64 streams x 4 drafts with scores 59 us (263 MB: 4.5 TB/s) + decide 4.8 + left over 15.1 + draw 6.7; one stream without scores 6.3 + 7.0, latency all of it (in cycles
 // of the draw: decide 5400, find the slice 3300, its weights 3200, walk 2600).
 #include "common.h"
 #include "kernels.h"
@@ -23,7 +23,7 @@ typedef float f32x4u_t __attribute__((ext_vector_type(4), aligned(4)));  // (row
 // exp(d) for -700 <= d <= 0: 2^k exp(r), k the nearest whole number to d / ln 2 (added to 1.5 2^52, where it is the low word), |r| <= ln 2 / 2, the polynomial of degree 10 through exp at the
 // Chebyshev nodes of that interval.  Relative error (checked against 60 digits on 4001 points): 4.3e-16 of the polynomial, i.e. two roundings, and 2.4e-17 |k| of the one-term reduction -- 1.7e-15
 // down to d = -40; over 128 k borders of an inverse CDF one draw in 10^9 could land elsewhere for it.  The score read is bound by these instructions, a 64-bit multiply-add an entry is 2.4 us of the
-// 84 that 64 streams x 4 drafts with scores take (degree 8, 1.05e-12: 80 -- but then uniforms 1e-12 beside a probability are decided wrongly).
+// 84 that 64 streams x 4 drafts with scores take (degree 8, 1.05e-12: 80 -- but then uniforms 1e-12 beside a probability are decided wrongly, relative to it).
 __device__ __forceinline__ double exp_core(double d) {
     const double t = fma(d, 1.4426950408889634074, 0x1.8p52), k = t - 0x1.8p52, r = fma(-k, 0.69314718055994530942, d);
     double p = 2.7626426376580335e-07;

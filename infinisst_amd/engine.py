@@ -782,7 +782,7 @@ def op_prefix_attention(q: torch.Tensor, k_prefix: torch.Tensor, v_prefix: torch
     tail_lens (seqs, int32) are live.  q (rows, heads, D): sequence b's newest positions are rows row_starts[b] .. row_starts[b + 1] - 1 (int32, seqs + 1; None: as many
     rows each); row t of n sees the prefix and the own keys 0 .. tail_lens[b] - n + t, a row without a key gives zeros, a row of no sequence is left as it was (in `out`;
     undefined without).  max_rows: most rows of one sequence if the caller knows it (speed only).  bf16, D 64 or 128, keys already rotated; strided views are fine while
-    rows are 16-byte aligned.  scale: default D ** -0.5."""
+    rows are 16-byte aligned (out: [rows][heads] or [heads][rows]).  Softmax weights enter the value product as bf16, all else is fp32.  scale: default D ** -0.5."""
     what = "op_prefix_attention"
     lib = _lib or load_library()
     dev = _device_of(what, q)
