@@ -371,7 +371,7 @@ def test_prefix_attention_values_near_the_end_of_the_range(rows, lens, P):
     q, kp, vp, kt, vt, ln, st = attn_inputs(35, rows, lens, 4, 2, 128, P, 96)
     at = torch.arange(P, device=DEV)
     q[..., 0], kt[..., 0] = 8.0, 0.0
-    kp[..., 0] = torch.where((at // 32 % 4 > 1) if max(rows) > 8 else (at >= 3072), 11.0, 0.0).to(BF)  # (two tiles low, two high; or every step of a wave but its first)
+    kp[..., 0] = torch.where((at // 32 % 4 > 1) if max(rows) > 8 else (at >= P // 2), 11.0, 0.0).to(BF)  # (two tiles low, two high; or the later steps of a wave)
     vp2, vt2 = vp.abs() * 2.0 ** 116, vt.abs() * 2.0 ** 116
     o, A = attn_ref(q, kp, vp2, kt, vt2, ln, st)
     got = E.op_prefix_attention(q, kp, vp2, kt, vt2, ln, st, max(rows)).cpu().double()
